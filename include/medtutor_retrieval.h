@@ -263,6 +263,63 @@ void mtr_multi_index_destroy(mtr_multi_index_t* index);
 int mtr_pool_normalize(const void* dev_hidden, int32_t dtype, const int64_t* dev_mask, int32_t b,
                        int32_t t, int32_t d, float* dev_out, int32_t device_id, void* stream);
 
+/* ---- the scoring head: a language model's last steps ------------------------
+ * For re-ranking retrieved pages by what a causal language model makes of them
+ * (the reference asks its inference engine for answer tokens' log probabilities,
+ * pipeline/utils/vllm_handler.py:109-144): final norm, product with the
+ * vocabulary matrix, log probabilities.  The decoder's body stays in PyTorch, as
+ * the encoder does.  Every call is enqueued on `stream` of GPU device_id without
+ * synchronising and allocates nothing, so all of them can be captured into HIP
+ * graphs; device pointers throughout.  Float types: MTR_F32, MTR_BF16, MTR_F16.
+ * Row strides (ld*) are in elements.  No rows (n == 0) is no error.
+ *
+ * Microscaled rows: blocks of MTR_MX_BLOCK consecutive elements share a
+ * power-of-two scale.  A row of d elements is padded with zeros to a multiple of
+ * MTR_MX_PAD; stored are
+ *   values  row-major, dense: MTR_MX_FP4 two e2m1 elements a byte (the earlier one
+ *           in the low half), MTR_MX_FP8 one e4m3 element a byte; on 16 bytes
+ *   scales  one byte a block, row-major, dense: exponent with bias 127; 255 marks a
+ *           block that held a NaN or infinity and reads back as NaN; on 4 bytes
+ * The scale is the smallest 2^s (s >= -127) under which the block's largest
+ * magnitude rounds to the largest element (6 and 448) or less; elements are
+ * rounded to nearest, ties to even. */
+enum { MTR_MX_FP4 = 0, MTR_MX_FP8 = 1 };
+#define MTR_MX_BLOCK 32
+#define MTR_MX_PAD 128
+int mtr_mx_quantize(const void* dev_x, int32_t dtype, int64_t n, int32_t d, int64_t ld, int32_t format,
+                    void* dev_values, void* dev_scales, int32_t device_id, void* stream);
+int mtr_mx_dequantize(const void* dev_values, const void* dev_scales, int32_t format, int64_t n, int32_t d,
+                      void* dev_out, int32_t dtype, int64_t ld, int32_t device_id, void* stream);
+/* h = x + residual, rounded to their type and written to dev_residual_out (dense
+ * rows; it may be the residual's own memory when that is dense); then
+ * h / sqrt(mean(h^2) + eps) * weight as microscaled rows.  dev_residual and
+ * dev_residual_out both NULL: h = x.  weight: d elements of the rows' type or
+ * fp32.  d <= MTR_RMS_NORM_MAX_WIDTH. */
+#define MTR_RMS_NORM_MAX_WIDTH 65536
+int mtr_rms_norm_mx(const void* dev_x, const void* dev_residual, const void* dev_weight, int32_t dtype,
+                    int32_t weight_dtype, int64_t n, int32_t d, int64_t ld_x, int64_t ld_residual, float eps,
+                    int32_t format, void* dev_residual_out, void* dev_values, void* dev_scales,
+                    int32_t device_id, void* stream);
+/* out[m][n] = A (m rows of d, either format) times the transpose of B (n rows of d,
+ * MTR_MX_FP4), MTR_F32 or MTR_BF16. */
+int mtr_mx_matmul(const void* dev_a_values, const void* dev_a_scales, int32_t a_format, int64_t m,
+                  const void* dev_b_values, const void* dev_b_scales, int64_t n, int32_t d, void* dev_out,
+                  int32_t out_dtype, int64_t ld_out, int32_t device_id, void* stream);
+/* Of n rows of v logits: the log probabilities [n][n_tokens] of tokens [n][n_tokens],
+ * the entropy [n] (nats), and the top_k (<= MTR_MAX_ALTERNATIVES) best tokens with
+ * their log probabilities, ordered by (logit descending, id ascending).  Logits of
+ * -inf are excluded: log probability -inf, never an alternative; slots beyond the
+ * tokens that are left hold id -1 and -inf.  A row with nothing left has entropy 0.
+ * A row that holds a NaN or +inf has NaN everywhere and ids -1.  A negative token
+ * is padding (0), one >= v gives NaN.  Workspace: mtr_token_logprobs_workspace
+ * bytes on 8 bytes, the caller's, not shared by calls that may overlap. */
+#define MTR_MAX_ALTERNATIVES 64
+int64_t mtr_token_logprobs_workspace(int64_t n, int64_t v, int32_t top_k);
+int mtr_token_logprobs(const void* dev_logits, int32_t dtype, int64_t n, int64_t v, int64_t ld,
+                       const int64_t* dev_tokens, int32_t n_tokens, int32_t top_k, float* dev_logprobs,
+                       float* dev_entropy, int64_t* dev_top_ids, float* dev_top_logprobs, void* dev_workspace,
+                       int64_t workspace_bytes, int32_t device_id, void* stream);
+
 /* Reader of the reference's index file, host side only (no GPU): one JSON
  * list of page objects, each with an "embedding" array of d numbers
  * (written at pipeline/utils/embed.py:74-79,110-113).  Takes over the json.load

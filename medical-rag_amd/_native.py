@@ -19,6 +19,10 @@ MTR_F32, MTR_F64, MTR_BF16, MTR_F16 = 0, 1, 2, 3
 MTR_ROWS_AS_STORED = 256
 MTR_COSINE, MTR_IP = 0, 1
 MTR_MAX_K = 1024
+MTR_MX_FP4, MTR_MX_FP8 = 0, 1
+MTR_MX_BLOCK, MTR_MX_PAD = 32, 128
+MTR_RMS_NORM_MAX_WIDTH = 65536
+MTR_MAX_ALTERNATIVES = 64
 
 MTR_EXCHANGE_AUTO, MTR_EXCHANGE_COPY, MTR_EXCHANGE_RCCL = 0, 1, 2
 EXCHANGES = {"auto": MTR_EXCHANGE_AUTO, "copy": MTR_EXCHANGE_COPY, "rccl": MTR_EXCHANGE_RCCL}
@@ -57,6 +61,12 @@ SIGNATURES = {
     "mtr_multi_index_read_rows": (_i32, [_vp, _i64, _i64, _vp]),
     "mtr_multi_index_destroy": (None, [_vp]),
     "mtr_pool_normalize": (_i32, [_vp, _i32, _vp, _i32, _i32, _i32, _vp, _i32, _vp]),
+    "mtr_mx_quantize": (_i32, [_vp, _i32, _i64, _i32, _i64, _i32, _vp, _vp, _i32, _vp]),
+    "mtr_mx_dequantize": (_i32, [_vp, _vp, _i32, _i64, _i32, _vp, _i32, _i64, _i32, _vp]),
+    "mtr_rms_norm_mx": (_i32, [_vp, _vp, _vp, _i32, _i32, _i64, _i32, _i64, _i64, C.c_float, _i32, _vp, _vp, _vp, _i32, _vp]),
+    "mtr_mx_matmul": (_i32, [_vp, _vp, _i32, _i64, _vp, _vp, _i64, _i32, _vp, _i32, _i64, _i32, _vp]),
+    "mtr_token_logprobs_workspace": (_i64, [_i64, _i64, _i32]),
+    "mtr_token_logprobs": (_i32, [_vp, _i32, _i64, _i64, _i64, _vp, _i32, _i32, _vp, _vp, _vp, _vp, _vp, _i64, _i32, _vp]),
     "mtr_index_info": (_i32, [_vp, C.POINTER(_i64), C.POINTER(_i32), C.POINTER(_i32), C.POINTER(_i32),
                               C.POINTER(_i32), C.POINTER(_i64)]),
     "mtr_index_read_rows": (_i32, [_vp, _i64, _i64, _vp]),

@@ -1,0 +1,254 @@
+// Rows to microscaled 4- and 8-bit floating point and back, and the root-mean-square
+// norm that writes such rows (mx_format.h says what they are).
+//
+// No counterpart in the reference: its encoder, re-ranker and index all stay in the
+// width the model library gives them (pipeline/utils/embed.py:64-79).
+#include "mx_format.h"
+
+namespace mtr {
+
+namespace {
+
+constexpr int kThreads = 256;
+
+template <int FMT> __device__ __forceinline__ void store_group(unsigned char* values, unsigned char* scales, long long group, int lane16,
+                                                               const unsigned int (&q)[FMT == kMxFp4 ? 1 : 2], unsigned int word) {
+    if constexpr (FMT == kMxFp4) {
+        reinterpret_cast<unsigned int*>(values)[group * 16 + lane16] = q[0];
+    } else {
+        reinterpret_cast<uint2*>(values)[group * 16 + lane16] = make_uint2(q[0], q[1]);
+    }
+    if (lane16 == 0) reinterpret_cast<unsigned int*>(scales)[group] = word;
+}
+
+// Groups of 128 elements, 16 lanes each.  VEC: rows start on 16 bytes and d is a
+// multiple of 8, so that every chunk of eight is whole or absent.
+template <typename T, int FMT, bool VEC>
+__global__ __launch_bounds__(kThreads) void mx_quantize_kernel(const T* __restrict__ x, unsigned int n_groups, unsigned int row_groups,
+                                                               int d, long long ld, unsigned char* __restrict__ values,
+                                                               unsigned char* __restrict__ scales) {
+    const unsigned int group = blockIdx.x * (kThreads / 16) + threadIdx.x / 16;
+    if (group >= n_groups) return;      // 16 lanes leave together
+    const int lane16 = threadIdx.x & 15;
+    const unsigned int row = group / row_groups;
+    const int col = (int)(group - row * row_groups) * 128 + lane16 * 8;
+    const T* p = x + (long long)row * ld + col;
+    float f[8];
+    if (VEC) {
+        if (col < d) load8<T>(p, f);
+        else
+#pragma unroll
+            for (int i = 0; i < 8; ++i) f[i] = 0.f;
+    } else {
+        load_some<T>(p, d - col, f);
+    }
+    unsigned int q[FMT == kMxFp4 ? 1 : 2];
+    const unsigned int word = mx_quantize8<FMT>(f, q);
+    store_group<FMT>(values, scales, group, lane16, q, word);
+}
+
+template <typename T, int FMT, bool VEC>
+__global__ __launch_bounds__(kThreads) void mx_dequantize_kernel(const unsigned char* __restrict__ values,
+                                                                 const unsigned char* __restrict__ scales, unsigned int n_groups,
+                                                                 unsigned int row_groups, int d, long long ld, T* __restrict__ out) {
+    const unsigned int group = blockIdx.x * (kThreads / 16) + threadIdx.x / 16;
+    if (group >= n_groups) return;
+    const int lane16 = threadIdx.x & 15;
+    const unsigned int row = group / row_groups;
+    const int col = (int)(group - row * row_groups) * 128 + lane16 * 8;
+    if (col >= d) return;
+    unsigned int q[FMT == kMxFp4 ? 1 : 2];
+    if constexpr (FMT == kMxFp4) {
+        q[0] = reinterpret_cast<const unsigned int*>(values)[(long long)group * 16 + lane16];
+    } else {
+        const uint2 w = reinterpret_cast<const uint2*>(values)[(long long)group * 16 + lane16];
+        q[0] = w.x;
+        q[1] = w.y;
+    }
+    float f[8];
+    mx_dequantize8<FMT>(q, reinterpret_cast<const unsigned int*>(scales)[group], f);
+    T* p = out + (long long)row * ld + col;
+    if (VEC) store8<T>(p, f);
+    else store_some<T>(p, d - col, f);
+}
+
+// y = h / sqrt(mean(h^2) + eps) * weight, h = x + residual, one workgroup of NT
+// threads a row, NC chunks of eight elements a thread, the row in registers
+// between the sum and the scaling: x and the residual are read once.  h is rounded
+// to the tensors' type (it is the residual stream that the next layer reads) and
+// the norm is taken of the rounded h, as a model that adds and norms in two steps
+// has it; the squares are summed in 32 bits.
+template <typename T, int FMT, int NT, int NC, bool RES, bool VEC>
+__global__ __launch_bounds__(NT) void rms_norm_mx_kernel(const T* __restrict__ x, const T* __restrict__ residual,
+                                                         const void* __restrict__ weight, int weight_f32, int d, long long ld_x,
+                                                         long long ld_res, float eps, T* __restrict__ residual_out,
+                                                         unsigned char* __restrict__ values, unsigned char* __restrict__ scales) {
+    __shared__ float red[NT / 64];
+    const long long row = blockIdx.x;
+    const int tid = threadIdx.x;
+    const T* px = x + row * ld_x;
+    const T* pr = RES ? residual + row * ld_res : nullptr;
+    float h[NC][8];
+    float ss = 0.f;
+#pragma unroll
+    for (int c = 0; c < NC; ++c) {
+        const int col = (c * NT + tid) * 8;
+        if (VEC && col < d) load8<T>(px + col, h[c]);
+        else load_some<T>(px + col, d - col, h[c]);
+    }
+    if constexpr (RES) {
+#pragma unroll
+        for (int c = 0; c < NC; ++c) {
+            const int col = (c * NT + tid) * 8;
+            float r[8];
+            if (VEC && col < d) load8<T>(pr + col, r);
+            else load_some<T>(pr + col, d - col, r);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) h[c][i] = to_f32<T>(from_f32<T>(h[c][i] + r[i]));
+            if (VEC && col < d) store8<T>(residual_out + row * d + col, h[c]);
+            else store_some<T>(residual_out + row * d + col, d - col, h[c]);
+        }
+    }
+#pragma unroll
+    for (int c = 0; c < NC; ++c)
+#pragma unroll
+        for (int i = 0; i < 8; ++i) ss = __builtin_fmaf(h[c][i], h[c][i], ss);
+#pragma unroll
+    for (int off = 32; off >= 1; off >>= 1) ss += __shfl_xor(ss, off, 64);
+    if constexpr (NT > 64) {
+        if ((tid & 63) == 0) red[tid >> 6] = ss;
+        __syncthreads();
+        ss = 0.f;
+#pragma unroll
+        for (int w = 0; w < NT / 64; ++w) ss += red[w];
+    }
+    const float inv = 1.f / sqrtf(ss / (float)d + eps);
+    const int padded = (d + kMxPad - 1) / kMxPad * kMxPad;
+    const long long group0 = row * (padded / 128);
+#pragma unroll
+    for (int c = 0; c < NC; ++c) {
+        const int col = (c * NT + tid) * 8;
+        if (col < padded) {             // 16 lanes decide alike
+            float w[8];
+            if (weight_f32) {
+                const float* pw = static_cast<const float*>(weight) + col;
+                if (VEC && col < d) load8<float>(pw, w);
+                else load_some<float>(pw, d - col, w);
+            } else {
+                const T* pw = static_cast<const T*>(weight) + col;
+                if (VEC && col < d) load8<T>(pw, w);
+                else load_some<T>(pw, d - col, w);
+            }
+#pragma unroll
+            for (int i = 0; i < 8; ++i) w[i] *= h[c][i] * inv;
+            unsigned int q[FMT == kMxFp4 ? 1 : 2];
+            const unsigned int word = mx_quantize8<FMT>(w, q);
+            store_group<FMT>(values, scales, group0 + col / 128, tid & 15, q, word);
+        }
+    }
+}
+
+template <typename T, int FMT>
+hipError_t quantize_typed(const void* x, long long n, int d, long long ld, void* values, void* scales, hipStream_t stream) {
+    const unsigned int row_groups = mx_padded(d) / 128, n_groups = (unsigned int)(n * row_groups);
+    const bool vec = d % 8 == 0 && (ld * sizeof(T)) % 16 == 0 && reinterpret_cast<uintptr_t>(x) % 16 == 0;
+    const dim3 grid((n_groups + kThreads / 16 - 1) / (kThreads / 16));
+    const T* p = static_cast<const T*>(x);
+    unsigned char *v = static_cast<unsigned char*>(values), *s = static_cast<unsigned char*>(scales);
+    if (vec) hipLaunchKernelGGL((mx_quantize_kernel<T, FMT, true>), grid, dim3(kThreads), 0, stream, p, n_groups, row_groups, d, ld, v, s);
+    else hipLaunchKernelGGL((mx_quantize_kernel<T, FMT, false>), grid, dim3(kThreads), 0, stream, p, n_groups, row_groups, d, ld, v, s);
+    return hipGetLastError();
+}
+
+template <typename T, int FMT>
+hipError_t dequantize_typed(const void* values, const void* scales, long long n, int d, void* out, long long ld, hipStream_t stream) {
+    const unsigned int row_groups = mx_padded(d) / 128, n_groups = (unsigned int)(n * row_groups);
+    const bool vec = d % 8 == 0 && (ld * sizeof(T)) % 16 == 0 && reinterpret_cast<uintptr_t>(out) % 16 == 0;
+    const dim3 grid((n_groups + kThreads / 16 - 1) / (kThreads / 16));
+    const unsigned char *v = static_cast<const unsigned char*>(values), *s = static_cast<const unsigned char*>(scales);
+    T* p = static_cast<T*>(out);
+    if (vec) hipLaunchKernelGGL((mx_dequantize_kernel<T, FMT, true>), grid, dim3(kThreads), 0, stream, v, s, n_groups, row_groups, d, ld, p);
+    else hipLaunchKernelGGL((mx_dequantize_kernel<T, FMT, false>), grid, dim3(kThreads), 0, stream, v, s, n_groups, row_groups, d, ld, p);
+    return hipGetLastError();
+}
+
+struct NormArgs {
+    const void *x, *residual, *weight;
+    int weight_f32;
+    long long n;
+    int d;
+    long long ld_x, ld_res;
+    float eps;
+    void *residual_out, *values, *scales;
+};
+
+template <typename T, int FMT, int NT, int NC, bool RES> hipError_t norm_shaped(const NormArgs& a, hipStream_t stream) {
+    const auto aligned = [](const void* p) { return reinterpret_cast<uintptr_t>(p) % 16 == 0; };
+    const bool vec = a.d % 8 == 0 && (a.ld_x * sizeof(T)) % 16 == 0 && aligned(a.x) && aligned(a.weight) &&
+                     (!RES || ((a.ld_res * sizeof(T)) % 16 == 0 && aligned(a.residual) && aligned(a.residual_out)));
+    const dim3 grid((unsigned int)a.n);
+#define MTR_NORM(V)                                                                                                                   \
+    hipLaunchKernelGGL((rms_norm_mx_kernel<T, FMT, NT, NC, RES, V>), grid, dim3(NT), 0, stream, static_cast<const T*>(a.x),              \
+                       static_cast<const T*>(a.residual), a.weight, a.weight_f32, a.d, a.ld_x, a.ld_res, a.eps,                        \
+                       static_cast<T*>(a.residual_out), static_cast<unsigned char*>(a.values), static_cast<unsigned char*>(a.scales))
+    if (vec) MTR_NORM(true);
+    else MTR_NORM(false);
+#undef MTR_NORM
+    return hipGetLastError();
+}
+
+// Threads a row: a wave up to 512 elements (nothing to exchange), then enough that a
+// thread holds at most 32 elements of rows up to 8192, and 64 beyond.
+template <typename T, int FMT, bool RES> hipError_t norm_typed(const NormArgs& a, hipStream_t stream) {
+    if (a.d <= 512) return norm_shaped<T, FMT, 64, 1, RES>(a, stream);
+    if (a.d <= 2048) return norm_shaped<T, FMT, 256, 1, RES>(a, stream);
+    if (a.d <= 4096) return norm_shaped<T, FMT, 256, 2, RES>(a, stream);
+    if (a.d <= 8192) return norm_shaped<T, FMT, 256, 4, RES>(a, stream);
+    return norm_shaped<T, FMT, 1024, 8, RES>(a, stream);
+}
+
+template <typename T> hipError_t norm_format(const NormArgs& a, int format, hipStream_t stream) {
+    if (format == kMxFp4) return a.residual ? norm_typed<T, kMxFp4, true>(a, stream) : norm_typed<T, kMxFp4, false>(a, stream);
+    return a.residual ? norm_typed<T, kMxFp8, true>(a, stream) : norm_typed<T, kMxFp8, false>(a, stream);
+}
+
+}  // namespace
+
+hipError_t launch_mx_quantize(const void* x, int dtype, long long n, int d, long long ld, int format, void* values, void* scales,
+                              hipStream_t stream) {
+#define MTR_BY_FORMAT(T) format == kMxFp4 ? quantize_typed<T, kMxFp4>(x, n, d, ld, values, scales, stream) : quantize_typed<T, kMxFp8>(x, n, d, ld, values, scales, stream)
+    switch (dtype) {
+        case 0: return MTR_BY_FORMAT(float);
+        case 2: return MTR_BY_FORMAT(bf16_t);
+        case 3: return MTR_BY_FORMAT(_Float16);
+        default: return hipErrorInvalidValue;
+    }
+#undef MTR_BY_FORMAT
+}
+
+hipError_t launch_mx_dequantize(const void* values, const void* scales, int format, long long n, int d, void* out, int dtype,
+                                long long ld, hipStream_t stream) {
+#define MTR_BY_FORMAT(T) format == kMxFp4 ? dequantize_typed<T, kMxFp4>(values, scales, n, d, out, ld, stream) : dequantize_typed<T, kMxFp8>(values, scales, n, d, out, ld, stream)
+    switch (dtype) {
+        case 0: return MTR_BY_FORMAT(float);
+        case 2: return MTR_BY_FORMAT(bf16_t);
+        case 3: return MTR_BY_FORMAT(_Float16);
+        default: return hipErrorInvalidValue;
+    }
+#undef MTR_BY_FORMAT
+}
+
+hipError_t launch_rms_norm_mx(const void* x, const void* residual, const void* weight, int dtype, int weight_dtype, long long n,
+                              int d, long long ld_x, long long ld_residual, float eps, int format, void* residual_out,
+                              void* values, void* scales, hipStream_t stream) {
+    if (d > kRmsNormMaxWidth || (weight_dtype != dtype && weight_dtype != 0)) return hipErrorInvalidValue;
+    const NormArgs a{x, residual, weight, weight_dtype == 0, n, d, ld_x, ld_residual, eps, residual_out, values, scales};
+    switch (dtype) {
+        case 0: return norm_format<float>(a, format, stream);
+        case 2: return norm_format<bf16_t>(a, format, stream);
+        case 3: return norm_format<_Float16>(a, format, stream);
+        default: return hipErrorInvalidValue;
+    }
+}
+
+}  // namespace mtr

@@ -1,0 +1,249 @@
+"""A causal language model's last steps on the GPU: final norm, vocabulary product
+in microscaled floating point, log probabilities.
+
+The reference re-ranks with the log probabilities that its inference engine
+returns for answer tokens (pipeline/utils/vllm_handler.py:109-144); rerank.py does
+it with these operators behind a decoder whose body stays a PyTorch(-ROCm)
+forward, as the encoder's does.
+
+    mx_quantize(x, format)                  -> MxRows        rows in blocks of 32 with a shared power-of-two scale
+    mx_dequantize(rows, dtype)              -> (n, d) tensor
+    rms_norm_mx(x, weight, eps, residual)   -> (MxRows, updated residual)
+    mx_matmul(a, b, dtype)                  -> (m, n) tensor, a's rows times b's
+    token_logprobs(logits, tokens, top_k)   -> TokenLogprobs
+
+Everything is enqueued on torch's current stream of the tensors' GPU without
+waiting, allocates through torch, and can be captured into a HIP graph.  The
+operators have no backward pass: they refuse inputs that record one.
+"""
+from __future__ import annotations
+
+from collections import namedtuple
+
+from . import _native
+
+__all__ = ["MxRows", "TokenLogprobs", "mx_quantize", "mx_dequantize", "rms_norm_mx", "mx_matmul", "token_logprobs"]
+
+FORMATS = {"mxfp4": _native.MTR_MX_FP4, "mxfp8": _native.MTR_MX_FP8}
+BLOCK, PAD = _native.MTR_MX_BLOCK, _native.MTR_MX_PAD
+
+TokenLogprobs = namedtuple("TokenLogprobs", "logprobs entropy top_ids top_logprobs")
+TokenLogprobs.__doc__ = """What token_logprobs returns: logprobs (n, g) and entropy (n,) float32, top_ids (n, top_k)
+int64, top_logprobs (n, top_k) float32."""
+
+_codes: dict = {}
+
+
+def _code(dtype, what):
+    """The library's code of a torch dtype it takes."""
+    if not _codes:
+        import torch
+        _codes.update({torch.float32: _native.MTR_F32, torch.bfloat16: _native.MTR_BF16, torch.float16: _native.MTR_F16})
+    try:
+        return _codes[dtype]
+    except KeyError:
+        raise TypeError(f"{what}: unsupported dtype {dtype}") from None
+
+
+def _stream(device):
+    import torch
+    return torch.cuda.current_stream(device).cuda_stream
+
+
+def _rows(x, what):
+    """A (n, d) GPU tensor with dense rows (copied if its last dimension is strided)."""
+    import torch
+    if not isinstance(x, torch.Tensor) or not x.is_cuda or x.dim() != 2:
+        raise ValueError(f"{what} wants a 2-D GPU tensor")
+    if x.requires_grad and torch.is_grad_enabled():
+        raise ValueError(f"{what} has no backward pass: detach its inputs or call it under torch.no_grad()")
+    return x if x.shape[1] < 2 or x.stride(1) == 1 else x.contiguous()
+
+
+def _width(d, format):
+    """(element bytes, scale bytes) of a stored row."""
+    padded = -(-d // PAD) * PAD
+    return (padded // 2 if format == "mxfp4" else padded), padded // BLOCK
+
+
+class MxRows:
+    """Rows in microscaled floating point, as include/medtutor_retrieval.h lays them
+    out: `values` (n, element bytes) and `scales` (n, scale bytes), uint8 tensors on
+    one GPU with dense rows, the number `d` of elements of a row, and the `format`,
+    "mxfp4" or "mxfp8"."""
+
+    __slots__ = ("values", "scales", "d", "format")
+
+    def __init__(self, values, scales, d: int, format: str = "mxfp4"):
+        import torch
+        if format not in FORMATS:
+            raise ValueError(f"format must be one of {sorted(FORMATS)}")
+        if d < 1:
+            raise ValueError("rows need at least one element")
+        for t in (values, scales):
+            if not isinstance(t, torch.Tensor) or not t.is_cuda or t.dtype != torch.uint8 or t.dim() != 2 or not t.is_contiguous():
+                raise ValueError("MxRows wants contiguous 2-D uint8 GPU tensors")
+        if values.device != scales.device:
+            raise ValueError(f"values are on {values.device}, scales on {scales.device}")
+        want = _width(d, format)
+        if (values.shape[1], scales.shape[1]) != want or values.shape[0] != scales.shape[0]:
+            raise ValueError(f"{format} rows of {d} elements have {want[0]} element and {want[1]} scale bytes, "
+                             f"got {tuple(values.shape)} and {tuple(scales.shape)}")
+        self.values, self.scales, self.d, self.format = values, scales, int(d), format
+
+    @classmethod
+    def empty(cls, n, d, format, device):
+        import torch
+        if format not in FORMATS:
+            raise ValueError(f"format must be one of {sorted(FORMATS)}")
+        if d < 1:
+            raise ValueError("rows need at least one element")
+        width, blocks = _width(d, format)
+        rows = cls.__new__(cls)
+        rows.values = torch.empty((n, width), dtype=torch.uint8, device=device)
+        rows.scales = torch.empty((n, blocks), dtype=torch.uint8, device=device)
+        rows.d, rows.format = int(d), format
+        return rows
+
+    def __len__(self):
+        return self.values.shape[0]
+
+    @property
+    def device(self):
+        return self.values.device
+
+    @property
+    def nbytes(self):
+        return self.values.numel() + self.scales.numel()
+
+    def rows(self, lo, hi):
+        """Rows [lo, hi) as a view."""
+        return MxRows(self.values[lo:hi], self.scales[lo:hi], self.d, self.format)
+
+    def __repr__(self):
+        return f"MxRows({len(self)} x {self.d}, {self.format}, {self.device})"
+
+
+def mx_quantize(x, format: str = "mxfp4") -> MxRows:
+    """(n, d) float32 / bfloat16 / float16 rows to microscaled floating point: blocks
+    of 32 with the smallest power-of-two scale under which the block's largest
+    magnitude rounds to the largest element or less, elements rounded to nearest,
+    ties to even.  A block that holds a NaN or infinity reads back as NaN."""
+    x = _rows(x, "mx_quantize")
+    n, d = x.shape
+    code = _code(x.dtype, "mx_quantize")
+    out = MxRows.empty(n, d, format, x.device)
+    _native.check(_native.lib().mtr_mx_quantize(x.data_ptr(), code, n, d, x.stride(0), FORMATS[format], out.values.data_ptr(),
+                                                out.scales.data_ptr(), x.device.index, _stream(x.device)))
+    return out
+
+
+def mx_dequantize(rows: MxRows, dtype=None, out=None):
+    """What microscaled rows stand for, as a (n, d) tensor of `dtype` (bfloat16, which
+    holds every value exactly but the very smallest, unless given) or into `out`, a
+    (n, d) GPU tensor with dense rows that do not overlap."""
+    import torch
+    n, d = len(rows), rows.d
+    if out is None:
+        code = _code(torch.bfloat16 if dtype is None else dtype, "mx_dequantize")
+        out = torch.empty((n, d), dtype=torch.bfloat16 if dtype is None else dtype, device=rows.device)
+    else:
+        code = _code(out.dtype, "mx_dequantize")
+        if out.shape != (n, d) or out.device != rows.device or (d > 1 and out.stride(1) != 1) or (dtype is not None and dtype != out.dtype):
+            raise ValueError("out must be a (n, d) tensor of the dtype on the rows' GPU, its rows dense")
+    _native.check(_native.lib().mtr_mx_dequantize(rows.values.data_ptr(), rows.scales.data_ptr(), FORMATS[rows.format], n, d,
+                                                  out.data_ptr(), code, out.stride(0), rows.device.index, _stream(rows.device)))
+    return out
+
+
+def rms_norm_mx(x, weight, eps: float = 1e-6, residual=None, format: str = "mxfp8"):
+    """Root-mean-square norm of x + residual, as microscaled rows: (MxRows, h) with
+    h = x + residual in their dtype (None without a residual), the rows
+    h / sqrt(mean(h^2) + eps) * weight.  x, residual: (n, d), one dtype; weight: (d,)
+    of that dtype or float32.  Sums are in 32 bits; d up to 65536."""
+    import torch
+    x = _rows(x, "rms_norm_mx")
+    n, d = x.shape
+    code = _code(x.dtype, "rms_norm_mx")
+    if (not isinstance(weight, torch.Tensor) or weight.shape != (d,) or weight.device != x.device
+            or weight.dtype not in (x.dtype, torch.float32)):
+        raise ValueError(f"rms_norm_mx wants a ({d},) weight of the rows' dtype or float32 on their GPU")
+    if weight.requires_grad and torch.is_grad_enabled():
+        raise ValueError("rms_norm_mx has no backward pass: detach its inputs or call it under torch.no_grad()")
+    weight = weight.contiguous()
+    h = None
+    if residual is not None:
+        residual = _rows(residual, "rms_norm_mx")
+        if residual.shape != x.shape or residual.dtype != x.dtype or residual.device != x.device:
+            raise ValueError("rms_norm_mx wants a residual of the rows' shape and dtype on their GPU")
+        h = torch.empty((n, d), dtype=x.dtype, device=x.device)
+    out = MxRows.empty(n, d, format, x.device)
+    _native.check(_native.lib().mtr_rms_norm_mx(
+        x.data_ptr(), residual.data_ptr() if h is not None else None, weight.data_ptr(), code, _code(weight.dtype, "rms_norm_mx"), n, d,
+        x.stride(0), residual.stride(0) if h is not None else 0, eps, FORMATS[format], h.data_ptr() if h is not None else None,
+        out.values.data_ptr(), out.scales.data_ptr(), x.device.index, _stream(x.device)))
+    return out, h
+
+
+def mx_matmul(a: MxRows, b: MxRows, dtype=None, out=None):
+    """(m, n) products of a's m rows (either format) with b's n rows (mxfp4), summed in
+    32 bits; float32 unless `dtype` says bfloat16, or into `out`, a (m, n) GPU tensor
+    with dense rows that do not overlap."""
+    import torch
+    if b.format != "mxfp4":
+        raise ValueError("mx_matmul wants its second operand in mxfp4")
+    if a.d != b.d:
+        raise ValueError(f"rows of {a.d} and of {b.d} elements")
+    if a.device != b.device:
+        raise ValueError(f"operands are on {a.device} and {b.device}")
+    m, n = len(a), len(b)
+    if out is None:
+        out = torch.empty((m, n), dtype=torch.float32 if dtype is None else dtype, device=a.device)
+    elif out.shape != (m, n) or out.device != a.device or (n > 1 and out.stride(1) != 1) or (dtype is not None and dtype != out.dtype):
+        raise ValueError("out must be a (m, n) tensor of the dtype on the operands' GPU, its rows dense")
+    if out.dtype not in (torch.float32, torch.bfloat16):
+        raise TypeError(f"mx_matmul: unsupported dtype {out.dtype}")
+    _native.check(_native.lib().mtr_mx_matmul(
+        a.values.data_ptr(), a.scales.data_ptr(), FORMATS[a.format], m, b.values.data_ptr(), b.scales.data_ptr(), n, a.d,
+        out.data_ptr(), _code(out.dtype, "mx_matmul"), out.stride(0), a.device.index, _stream(a.device)))
+    return out
+
+
+def token_logprobs(logits, tokens=None, top_k: int = 0) -> TokenLogprobs:
+    """Of (n, v) float32 / bfloat16 / float16 logits: the log probabilities of the given
+    tokens, (n,) or (n, g) int64, the entropy in nats, and the top_k (up to 64) best
+    tokens with theirs, ordered by (logit descending, id ascending).
+
+    Logits of -inf are excluded tokens: their log probability is -inf and they are no
+    alternatives; slots beyond the tokens that are left hold id -1 and -inf.  A row
+    with nothing left has entropy 0; one that holds a NaN or +inf has NaN everywhere.
+    A negative token is padding, its log probability 0; one >= v gives NaN (the call
+    does not wait for the GPU and so cannot raise)."""
+    import torch
+    logits = _rows(logits, "token_logprobs")
+    n, v = logits.shape
+    code = _code(logits.dtype, "token_logprobs")
+    device = logits.device
+    if tokens is None:
+        tokens = torch.empty((n, 0), dtype=torch.int64, device=device)
+    if not isinstance(tokens, torch.Tensor) or tokens.dtype != torch.int64 or tokens.device != device:
+        raise ValueError("token_logprobs wants int64 tokens on the logits' GPU")
+    if tokens.dim() == 1:
+        tokens = tokens[:, None]
+    if tokens.dim() != 2 or tokens.shape[0] != n:
+        raise ValueError(f"token_logprobs wants ({n},) or ({n}, g) tokens, got {tuple(tokens.shape)}")
+    if not 0 <= top_k <= _native.MTR_MAX_ALTERNATIVES:
+        raise ValueError(f"top_k must be in [0, {_native.MTR_MAX_ALTERNATIVES}]")
+    tokens = tokens.contiguous()
+    g = tokens.shape[1]
+    lib = _native.lib()
+    logprobs = torch.empty((n, g), dtype=torch.float32, device=device)
+    entropy = torch.empty(n, dtype=torch.float32, device=device)
+    top_ids = torch.empty((n, top_k), dtype=torch.int64, device=device)
+    top_logprobs = torch.empty((n, top_k), dtype=torch.float32, device=device)
+    need = lib.mtr_token_logprobs_workspace(n, v, top_k)
+    workspace = torch.empty(need, dtype=torch.uint8, device=device) if need else None
+    _native.check(lib.mtr_token_logprobs(
+        logits.data_ptr(), code, n, v, logits.stride(0), tokens.data_ptr(), g, top_k, logprobs.data_ptr(), entropy.data_ptr(),
+        top_ids.data_ptr(), top_logprobs.data_ptr(), workspace.data_ptr() if need else None, need, device.index, _stream(device)))
+    return TokenLogprobs(logprobs, entropy, top_ids, top_logprobs)
