@@ -301,10 +301,13 @@ int mtr_rms_norm_mx(const void* dev_x, const void* dev_residual, const void* dev
                     int32_t format, void* dev_residual_out, void* dev_values, void* dev_scales,
                     int32_t device_id, void* stream);
 /* out[m][n] = A (m rows of d, either format) times the transpose of B (n rows of d,
- * MTR_MX_FP4), MTR_F32 or MTR_BF16. */
+ * MTR_MX_FP4), MTR_F32 or MTR_BF16.  Workspace: mtr_mx_matmul_workspace bytes on 4
+ * bytes, the caller's, not shared by calls that may overlap. */
+int64_t mtr_mx_matmul_workspace(int64_t m, int64_t n, int32_t d);
 int mtr_mx_matmul(const void* dev_a_values, const void* dev_a_scales, int32_t a_format, int64_t m,
                   const void* dev_b_values, const void* dev_b_scales, int64_t n, int32_t d, void* dev_out,
-                  int32_t out_dtype, int64_t ld_out, int32_t device_id, void* stream);
+                  int32_t out_dtype, int64_t ld_out, void* dev_workspace, int64_t workspace_bytes,
+                  int32_t device_id, void* stream);
 /* Of n rows of v logits: the log probabilities [n][n_tokens] of tokens [n][n_tokens],
  * the entropy [n] (nats), and the top_k (<= MTR_MAX_ALTERNATIVES) best tokens with
  * their log probabilities, ordered by (logit descending, id ascending).  Logits of

@@ -64,7 +64,8 @@ SIGNATURES = {
     "mtr_mx_quantize": (_i32, [_vp, _i32, _i64, _i32, _i64, _i32, _vp, _vp, _i32, _vp]),
     "mtr_mx_dequantize": (_i32, [_vp, _vp, _i32, _i64, _i32, _vp, _i32, _i64, _i32, _vp]),
     "mtr_rms_norm_mx": (_i32, [_vp, _vp, _vp, _i32, _i32, _i64, _i32, _i64, _i64, C.c_float, _i32, _vp, _vp, _vp, _i32, _vp]),
-    "mtr_mx_matmul": (_i32, [_vp, _vp, _i32, _i64, _vp, _vp, _i64, _i32, _vp, _i32, _i64, _i32, _vp]),
+    "mtr_mx_matmul_workspace": (_i64, [_i64, _i64, _i32]),
+    "mtr_mx_matmul": (_i32, [_vp, _vp, _i32, _i64, _vp, _vp, _i64, _i32, _vp, _i32, _i64, _vp, _i64, _i32, _vp]),
     "mtr_token_logprobs_workspace": (_i64, [_i64, _i64, _i32]),
     "mtr_token_logprobs": (_i32, [_vp, _i32, _i64, _i64, _i64, _vp, _i32, _i32, _vp, _vp, _vp, _vp, _vp, _i64, _i32, _vp]),
     "mtr_index_info": (_i32, [_vp, C.POINTER(_i64), C.POINTER(_i32), C.POINTER(_i32), C.POINTER(_i32),

@@ -162,8 +162,10 @@ hipError_t launch_rms_norm_mx(const void* x, const void* residual, const void* w
                               void* values, void* scales, hipStream_t stream);
 
 // out[m][n] = A [m][k] times the transpose of B [n][k] (4-bit); out_dtype 0 fp32, 2 bf16.
+// workspace: mx_matmul_workspace bytes on 4 bytes (0: none is needed).
+long long mx_matmul_workspace(long long m, long long n, int d);
 hipError_t launch_mx_matmul(const void* a_values, const void* a_scales, int a_format, long long m, const void* b_values,
-                            const void* b_scales, long long n, int d, void* out, int out_dtype, long long ld_out,
+                            const void* b_scales, long long n, int d, void* out, int out_dtype, long long ld_out, void* workspace,
                             hipStream_t stream);
 
 // Scratch of launch_token_logprobs in bytes (0: none is needed).

@@ -9,7 +9,14 @@
 //     sums (2-norm error 6e-6 to 3e-5).
 //   v_mfma_f32_16x16x32_bf16 on both operands times their scales, which bfloat16 holds
 //     exactly: sums as exact as 32 bits allow, at half the rate and with the conversions.
-// 8-bit rows take the second, 4-bit rows the first.
+// 4-bit rows take the first.  8-bit rows take the second where few rows make the
+// product wait for memory anyway or the results are kept in 32 bits, and the first
+// where they are rounded to bfloat16, whose half step of 4e-3 is a hundred times the
+// difference.
+//
+// Two kernels.  Up to kFewRows rows of A the product is bound by the one pass over B: every wave
+// takes 16 rows of B straight from memory into its operand registers.  More rows
+// take tiles staged in LDS.
 #include "mx_format.h"
 
 namespace mtr {
@@ -20,6 +27,8 @@ using i32x8 = __attribute__((ext_vector_type(8))) int;
 using i32x4 = __attribute__((ext_vector_type(4))) int;
 using bf16x8 = __attribute__((ext_vector_type(8))) __bf16;
 using bf16x2 = __attribute__((ext_vector_type(2))) __bf16;
+typedef __attribute__((address_space(3))) void* lds_ptr_t;
+typedef const __attribute__((address_space(1))) void* gbl_ptr_t;
 
 // Eight 4-bit elements (a word) times the scale.
 __device__ __forceinline__ bf16x8 widen_fp4(unsigned int w, float scale) {
@@ -34,25 +43,38 @@ __device__ __forceinline__ bf16x8 widen_fp8(unsigned int lo, unsigned int hi, fl
     return bf16x8{a[0], a[1], b[0], b[1], c[0], c[1], d[0], d[1]};
 }
 
+template <typename T> struct alignas(4 * sizeof(T)) Four { T v[4]; };
+
+// Four neighbouring results.  whole: all of them exist and their address is a multiple of their size.
+template <typename T> __device__ __forceinline__ void store4(T* p, long long left, bool whole, const f32x4& v) {
+    if (whole && left >= 4) {
+        Four<T> o;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) o.v[i] = from_f32<T>(v[i]);
+        *reinterpret_cast<Four<T>*>(p) = o;
+    } else {
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+            if (i < left) p[i] = from_f32<T>(v[i]);
+    }
+}
+
+// ---- few rows of A -----------------------------------------------------------------
+
 struct MatmulArgs {
     const unsigned char *a, *a_scales, *b, *b_scales;
     long long m, n;
     int groups;         // of 128 elements a row
     void* out;
     long long ld;
+    int whole;          // four neighbouring results can be stored at once
 };
 
-template <typename T> __device__ __forceinline__ void store4(T* p, long long left, const f32x4& v) {
-#pragma unroll
-    for (int i = 0; i < 4; ++i)
-        if (i < left) p[i] = from_f32<T>(v[i]);
-}
-
-// One wave 16 x 16 outputs, operands straight from memory.  Rows of B are the
+// One wave 16 rows of B times 16 of A, operands straight from memory.  Rows of B are the
 // instruction's rows, so that a lane ends with four neighbouring columns of out.  A lane
 // holds block lane / 16 of row lane % 16 of each 128: its scale is one byte.
 template <int FA, typename TO>
-__global__ __launch_bounds__(256) void mx_matmul_kernel(MatmulArgs p) {
+__global__ __launch_bounds__(256) void mx_matmul_rows_kernel(MatmulArgs p) {
     const int lane = threadIdx.x & 63, r = lane & 15, g = lane >> 4;
     const long long n0 = ((long long)blockIdx.x * 4 + (threadIdx.x >> 6)) * 16, m0 = (long long)blockIdx.y * 16;
     if (n0 >= p.n) return;
@@ -79,19 +101,274 @@ __global__ __launch_bounds__(256) void mx_matmul_kernel(MatmulArgs p) {
             acc = __builtin_amdgcn_mfma_f32_16x16x32_bf16(widen_fp4(vb[3], fb), widen_fp8(v1[2], v1[3], fa), acc, 0, 0, 0);
         }
     }
-    if (m0 + r < p.m) store4<TO>(static_cast<TO*>(p.out) + (m0 + r) * p.ld + n0 + 4 * g, p.n - n0 - 4 * g, acc);
+    if (m0 + r < p.m)
+        store4<TO>(static_cast<TO*>(p.out) + (m0 + r) * p.ld + n0 + 4 * g, p.n - n0 - 4 * g, p.whole, acc);
+}
+
+// ---- tiles ---------------------------------------------------------------------------
+
+constexpr int kTileThreads = 512, kTileN = 256, kStages = 3;
+
+// Scale words (the four scale bytes of 128 elements) turned from [rows][groups] to
+// [groups][padded rows], where a tile's words of one K step lie together: read where
+// they are, each row's four bytes would cost a request of their own, as many as the
+// elements' do.
+__global__ __launch_bounds__(256) void turn_scales_kernel(const unsigned int* __restrict__ src, long long rows, int groups,
+                                                          long long padded_rows, unsigned int* __restrict__ dst) {
+    __shared__ unsigned int tile[32][65];
+    const long long r0 = (long long)blockIdx.x * 64;
+    const int g0 = blockIdx.y * 32;
+    for (int i = threadIdx.x; i < 64 * 32; i += 256) {
+        const int r = i / 32, g = i % 32;
+        if (r0 + r < rows && g0 + g < groups) tile[g][r] = src[(r0 + r) * groups + g0 + g];
+    }
+    __syncthreads();
+    for (int i = threadIdx.x; i < 64 * 32; i += 256) {
+        const int g = i / 64, r = i % 64;
+        if (r0 + r < rows && g0 + g < groups) dst[(long long)(g0 + g) * padded_rows + r0 + r] = tile[g][r];
+    }
+}
+
+struct TileArgs {
+    const unsigned char *a, *b;
+    const unsigned int *a_scales, *b_scales;    // turned: [groups][padded rows]
+    long long m, n, m_padded, n_padded;
+    int groups;
+    int m_tiles;
+    void* out;
+    long long ld;
+    int whole;
+};
+
+__device__ __forceinline__ const unsigned char* scalar_pointer(const unsigned char* p) {
+    const unsigned long long v = reinterpret_cast<unsigned long long>(p);
+    const unsigned int lo = __builtin_amdgcn_readfirstlane((unsigned int)v);
+    const unsigned int hi = __builtin_amdgcn_readfirstlane((unsigned int)(v >> 32));
+    return reinterpret_cast<const unsigned char*>(((unsigned long long)hi << 32) | lo);
+}
+
+// s_barrier without the drain of outstanding loads that __syncthreads() adds.
+__device__ __forceinline__ void barrier_keeping_loads() {
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
+}
+
+// A tile of 64 WM rows of A times 256 rows of B; eight waves, WM x (8 / WM), each 64 rows
+// of A times 32 WM of B.  K steps of 128 elements in a ring of three LDS stages, filled
+// by 16-byte direct-to-LDS loads two steps ahead; one barrier a step.  A wave waits for its
+// own loads of step s (all but the newest step's), the barrier then says that everybody's
+// have landed, and that everybody is done with step s - 1, whose stage step s + 2 takes.
+// 16-byte chunks are swizzled on the loads' source addresses so that the 16 rows that a
+// quarter wave reads at once start in different banks.
+template <int FA, bool EXACT, int WM> struct Tile {
+    static constexpr int M = 64 * WM, WN = 8 / WM, NT = kTileN / WN / 16, MT = 4;
+    static constexpr int kRowA = FA == kMxFp4 ? 64 : 128;       // bytes of a row of A a step
+    static constexpr int kBytesA = M * kRowA, kBytesB = kTileN * 64;
+    static constexpr int kStage = kBytesA + kBytesB + 2048;     // 512 scale words: A's M, B's 256, the rest unused
+    static constexpr int kLoadsA = kBytesA / 8192, kLoadsB = kBytesB / 8192, kLoads = kLoadsA + kLoadsB + 1;
+};
+
+template <int FA, bool EXACT, int WM, typename TO>
+__global__ __launch_bounds__(kTileThreads, 2) void mx_matmul_tile_kernel(TileArgs p) {
+    using S = Tile<FA, EXACT, WM>;
+    extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
+    const int lane = threadIdx.x & 63, r = lane & 15, g = lane >> 4;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int wm = wave / S::WN, wn = wave % S::WN;
+    // workgroups of one XCD take consecutive tiles, A's running fastest: they share rows of B in its L2
+    const int nwg = gridDim.x, xcd = blockIdx.x % 8, per = nwg / 8, rem = nwg % 8;
+    const int id = (xcd < rem ? xcd * (per + 1) : rem * (per + 1) + (xcd - rem) * per) + blockIdx.x / 8;
+    const long long m0 = (long long)(id % p.m_tiles) * S::M, n0 = (long long)(id / p.m_tiles) * kTileN;
+
+    const unsigned int row_a = p.groups * S::kRowA, row_b = p.groups * 64;
+    const unsigned char* a0 = p.a + m0 * row_a;
+    const unsigned char* b0 = p.b + n0 * row_b;
+    const int last_a = (int)(p.m - 1 - m0 < S::M - 1 ? p.m - 1 - m0 : S::M - 1);
+    const int last_b = (int)(p.n - 1 - n0 < kTileN - 1 ? p.n - 1 - n0 : kTileN - 1);
+    unsigned int off_a[S::kLoadsA], off_b[S::kLoadsB];
+#pragma unroll
+    for (int i = 0; i < S::kLoadsA; ++i) {
+        const int piece = wave * S::kLoadsA + i;        // 1 KiB
+        const int row = FA == kMxFp4 ? piece * 16 + lane / 4 : piece * 8 + lane / 8;
+        const int chunk = FA == kMxFp4 ? (lane & 3) ^ ((lane >> 4) & 3) : (lane & 7) ^ (lane >> 3);
+        off_a[i] = (unsigned int)(row < last_a ? row : last_a) * row_a + chunk * 16;
+    }
+#pragma unroll
+    for (int i = 0; i < S::kLoadsB; ++i) {
+        const int row = (wave * S::kLoadsB + i) * 16 + lane / 4;
+        off_b[i] = (unsigned int)(row < last_b ? row : last_b) * row_b + ((lane & 3) ^ ((lane >> 4) & 3)) * 16;
+    }
+    // wave w loads the scale words of rows 64 w ..: A's first, then B's (the last of them again where there are fewer)
+    const int srow = wave * 64;
+    const unsigned char* s0;
+    long long s_step;
+    if (srow < S::M) {
+        s0 = reinterpret_cast<const unsigned char*>(p.a_scales + m0 + srow);
+        s_step = p.m_padded * 4;
+    } else {
+        const int over = srow - S::M < kTileN ? srow - S::M : kTileN - 64;
+        s0 = reinterpret_cast<const unsigned char*>(p.b_scales + n0 + over);
+        s_step = p.n_padded * 4;
+    }
+    auto request = [&](int k, unsigned char* dst) {
+        const unsigned char* a = scalar_pointer(a0 + (long long)k * S::kRowA);
+        const unsigned char* b = scalar_pointer(b0 + (long long)k * 64);
+        const unsigned char* s = scalar_pointer(s0 + k * s_step);
+#pragma unroll
+        for (int i = 0; i < S::kLoadsA; ++i)
+            __builtin_amdgcn_global_load_lds((gbl_ptr_t)(a + off_a[i]), (lds_ptr_t)(dst + (wave * S::kLoadsA + i) * 1024), 16, 0, 0);
+#pragma unroll
+        for (int i = 0; i < S::kLoadsB; ++i)
+            __builtin_amdgcn_global_load_lds((gbl_ptr_t)(b + off_b[i]), (lds_ptr_t)(dst + S::kBytesA + (wave * S::kLoadsB + i) * 1024), 16, 0, 0);
+        __builtin_amdgcn_global_load_lds((gbl_ptr_t)(s + lane * 4), (lds_ptr_t)(dst + S::kBytesA + S::kBytesB + wave * 256), 4, 0, 0);
+    };
+
+    f32x4 acc[S::NT][S::MT];
+#pragma unroll
+    for (int i = 0; i < S::NT; ++i)
+#pragma unroll
+        for (int j = 0; j < S::MT; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+
+    request(0, smem);
+    request(p.groups > 1 ? 1 : 0, smem + S::kStage);
+    int now = 0;
+    for (int k = 0; k < p.groups; ++k) {
+        asm volatile("s_waitcnt vmcnt(%0)" ::"n"(S::kLoads) : "memory");
+        barrier_keeping_loads();
+        const int next = now == 0 ? 2 : now - 1;        // (now + 2) % 3
+        request(k + 2 < p.groups ? k + 2 : p.groups - 1, smem + next * S::kStage);
+        const unsigned char* st = smem + now * S::kStage;
+        now = now == 2 ? 0 : now + 1;
+        const unsigned char* sa = st + wm * 64 * S::kRowA;
+        const unsigned char* sb = st + S::kBytesA + wn * S::NT * 16 * 64;
+        const unsigned int* sca = reinterpret_cast<const unsigned int*>(st + S::kBytesA + S::kBytesB) + wm * 64;
+        const unsigned int* scb = reinterpret_cast<const unsigned int*>(st + S::kBytesA + S::kBytesB) + S::M + wn * S::NT * 16;
+        unsigned int xa[S::MT], xb[S::NT];
+#pragma unroll
+        for (int j = 0; j < S::MT; ++j) xa[j] = sca[j * 16 + r] >> (8 * g);
+#pragma unroll
+        for (int i = 0; i < S::NT; ++i) xb[i] = scb[i * 16 + r] >> (8 * g);
+        if constexpr (!EXACT) {
+            i32x8 fa[S::MT];
+#pragma unroll
+            for (int j = 0; j < S::MT; ++j) {
+                const unsigned char* row = sa + (j * 16 + r) * S::kRowA;
+                if constexpr (FA == kMxFp4) {
+                    const i32x4 v = *reinterpret_cast<const i32x4*>(row + ((g ^ ((r >> 2) & 3)) << 4));
+                    fa[j] = __builtin_shufflevector(v, v, 0, 1, 2, 3, -1, -1, -1, -1);
+                } else {        // the instruction takes elements 16 g .. and 64 + 16 g .. of an 8-bit row
+                    const i32x4 v = *reinterpret_cast<const i32x4*>(row + ((g ^ (r & 7)) << 4));
+                    const i32x4 w = *reinterpret_cast<const i32x4*>(row + (((4 + g) ^ (r & 7)) << 4));
+                    fa[j] = __builtin_shufflevector(v, w, 0, 1, 2, 3, 4, 5, 6, 7);
+                }
+            }
+#pragma unroll
+            for (int i = 0; i < S::NT; ++i) {
+                const i32x4 v = *reinterpret_cast<const i32x4*>(sb + (i * 16 + r) * 64 + ((g ^ ((r >> 2) & 3)) << 4));
+                const i32x8 fb = __builtin_shufflevector(v, v, 0, 1, 2, 3, -1, -1, -1, -1);
+#pragma unroll
+                for (int j = 0; j < S::MT; ++j)
+                    acc[i][j] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(fb, fa[j], acc[i][j], 4, FA == kMxFp4 ? 4 : 0, 0,
+                                                                                 (int)xb[i], 0, (int)xa[j]);
+            }
+        } else {
+            // elements 32 g .. of both, eight at a time
+            u32x4 va[S::MT][2];
+#pragma unroll
+            for (int j = 0; j < S::MT; ++j) {
+                const unsigned char* row = sa + (j * 16 + r) * S::kRowA;
+                va[j][0] = *reinterpret_cast<const u32x4*>(row + (((2 * g) ^ (r & 7)) << 4));
+                va[j][1] = *reinterpret_cast<const u32x4*>(row + (((2 * g + 1) ^ (r & 7)) << 4));
+            }
+            u32x4 vb[S::NT];
+#pragma unroll
+            for (int i = 0; i < S::NT; ++i) vb[i] = *reinterpret_cast<const u32x4*>(sb + (i * 16 + r) * 64 + ((g ^ ((r >> 2) & 3)) << 4));
+#pragma unroll
+            for (int h = 0; h < 4; ++h) {
+                bf16x8 fa[S::MT];
+#pragma unroll
+                for (int j = 0; j < S::MT; ++j) fa[j] = widen_fp8(va[j][h / 2][(h % 2) * 2], va[j][h / 2][(h % 2) * 2 + 1], mx_scale(xa[j] & 255u));
+#pragma unroll
+                for (int i = 0; i < S::NT; ++i) {
+                    const bf16x8 fb = widen_fp4(vb[i][h], mx_scale(xb[i] & 255u));
+#pragma unroll
+                    for (int j = 0; j < S::MT; ++j) acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(fb, fa[j], acc[i][j], 0, 0, 0);
+                }
+            }
+        }
+    }
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");    // the loads past the last step still write to this workgroup's LDS
+#pragma unroll
+    for (int j = 0; j < S::MT; ++j) {
+        const long long row = m0 + wm * 64 + j * 16 + r;
+        if (row >= p.m) continue;
+        TO* o = static_cast<TO*>(p.out) + row * p.ld;
+#pragma unroll
+        for (int i = 0; i < S::NT; ++i) {
+            const long long col = n0 + (wn * S::NT + i) * 16 + 4 * g;
+            store4<TO>(o + col, p.n - col, p.whole, acc[i][j]);
+        }
+    }
+}
+
+constexpr int kFewRows = 64;
+constexpr int kTileMaxGroups = 16384;       // offsets within a tile fit 32 bits
+
+bool takes_tiles(long long m, int groups) { return m > kFewRows && groups <= kTileMaxGroups; }
+long long up(long long x, long long to) { return (x + to - 1) / to * to; }
+
+template <int FA, bool EXACT, int WM, typename TO> hipError_t launch_tiles(TileArgs p, hipStream_t stream) {
+    using S = Tile<FA, EXACT, WM>;
+    constexpr int lds = kStages * S::kStage;
+    const void* fn = reinterpret_cast<const void*>(&mx_matmul_tile_kernel<FA, EXACT, WM, TO>);
+    static_assert(lds <= 160 * 1024, "LDS");
+    const hipError_t e = hipFuncSetAttribute(fn, hipFuncAttributeMaxDynamicSharedMemorySize, lds);
+    if (e != hipSuccess) return e;
+    p.m_tiles = (int)((p.m + S::M - 1) / S::M);
+    const long long tiles = p.m_tiles * ((p.n + kTileN - 1) / kTileN);
+    if (tiles > 0x7fffffff) return hipErrorInvalidValue;
+    hipLaunchKernelGGL((mx_matmul_tile_kernel<FA, EXACT, WM, TO>), dim3((unsigned int)tiles), dim3(kTileThreads), lds, stream, p);
+    return hipGetLastError();
 }
 
 }  // namespace
 
+long long mx_matmul_workspace(long long m, long long n, int d) {
+    const int groups = mx_padded(d) / 128;
+    return takes_tiles(m, groups) ? (up(m, 256) + up(n, 256)) * groups * 4 : 0;
+}
+
 hipError_t launch_mx_matmul(const void* a_values, const void* a_scales, int a_format, long long m, const void* b_values,
-                            const void* b_scales, long long n, int d, void* out, int out_dtype, long long ld_out,
+                            const void* b_scales, long long n, int d, void* out, int out_dtype, long long ld_out, void* workspace,
                             hipStream_t stream) {
-    const MatmulArgs p{static_cast<const unsigned char*>(a_values), static_cast<const unsigned char*>(a_scales),
-                       static_cast<const unsigned char*>(b_values), static_cast<const unsigned char*>(b_scales), m, n,
-                       mx_padded(d) / 128, out, ld_out};
+    const int groups = mx_padded(d) / 128;
+    const size_t size = out_dtype == 0 ? 4 : 2;
+    const int whole = ld_out % 4 == 0 && reinterpret_cast<uintptr_t>(out) % (4 * size) == 0;
+    const auto* a = static_cast<const unsigned char*>(a_values);
+    const auto* b = static_cast<const unsigned char*>(b_values);
+    if (takes_tiles(m, groups)) {
+        unsigned int* as = static_cast<unsigned int*>(workspace);
+        unsigned int* bs = as + up(m, 256) * groups;
+        const auto turn = [&](const void* src, long long rows, unsigned int* dst) {
+            const dim3 grid((unsigned int)((rows + 63) / 64), (unsigned int)((groups + 31) / 32));
+            hipLaunchKernelGGL(turn_scales_kernel, grid, dim3(256), 0, stream, static_cast<const unsigned int*>(src), rows, groups, up(rows, 256), dst);
+        };
+        turn(a_scales, m, as);
+        turn(b_scales, n, bs);
+        const TileArgs p{a, b, as, bs, m, n, up(m, 256), up(n, 256), groups, 0, out, ld_out, whole};
+#define MTR_TILES(F, X, T) return m <= 128 ? launch_tiles<F, X, 2, T>(p, stream) : launch_tiles<F, X, 4, T>(p, stream)
+        if (a_format == kMxFp4) {
+            if (out_dtype == 0) MTR_TILES(kMxFp4, false, float);
+            MTR_TILES(kMxFp4, false, bf16_t);
+        }
+        if (out_dtype == 0) MTR_TILES(kMxFp8, true, float);
+        MTR_TILES(kMxFp8, false, bf16_t);
+#undef MTR_TILES
+    }
+    const MatmulArgs p{a, static_cast<const unsigned char*>(a_scales), b, static_cast<const unsigned char*>(b_scales), m, n, groups, out, ld_out, whole};
     const dim3 grid((unsigned int)((n + 63) / 64), (unsigned int)((m + 15) / 16));
-#define MTR_MATMUL(F, T) hipLaunchKernelGGL((mx_matmul_kernel<F, T>), grid, dim3(256), 0, stream, p)
+#define MTR_MATMUL(F, T) hipLaunchKernelGGL((mx_matmul_rows_kernel<F, T>), grid, dim3(256), 0, stream, p)
     if (out_dtype == 0) {
         if (a_format == kMxFp4) MTR_MATMUL(kMxFp4, float);
         else MTR_MATMUL(kMxFp8, float);

@@ -104,9 +104,14 @@ int mtr_rms_norm_mx(const void* dev_x, const void* dev_residual, const void* dev
                                             dev_residual_out, dev_values, dev_scales, static_cast<hipStream_t>(stream)));
 }
 
+int64_t mtr_mx_matmul_workspace(int64_t m, int64_t n, int32_t d) {
+    if (m < 1 || n < 1 || d < 1 || d > kMost - MTR_MX_PAD || m > kMost || n > kMost) return 0;
+    return mtr::mx_matmul_workspace(m, n, d);
+}
+
 int mtr_mx_matmul(const void* dev_a_values, const void* dev_a_scales, int32_t a_format, int64_t m, const void* dev_b_values,
                   const void* dev_b_scales, int64_t n, int32_t d, void* dev_out, int32_t out_dtype, int64_t ld_out,
-                  int32_t device_id, void* stream) {
+                  void* dev_workspace, int64_t workspace_bytes, int32_t device_id, void* stream) {
     if (out_dtype != MTR_F32 && out_dtype != MTR_BF16) return set_error(MTR_ERR_INVALID, "bad output dtype %d", out_dtype);
     if (int rc = check_rows("mtr_mx_matmul", m, d, dev_a_values, dev_a_scales, a_format)) return rc;
     if (int rc = check_rows("mtr_mx_matmul", n, d, dev_b_values, dev_b_scales, MTR_MX_FP4)) return rc;
@@ -114,10 +119,13 @@ int mtr_mx_matmul(const void* dev_a_values, const void* dev_a_scales, int32_t a_
     if (!dev_out) return set_error(MTR_ERR_INVALID, "NULL argument");
     if (off(dev_out, size_of(out_dtype)) || (m > 1 && ld_out < n))
         return set_error(MTR_ERR_INVALID, "bad row stride %lld or address", (long long)ld_out);
+    const int64_t need = mtr::mx_matmul_workspace(m, n, d);
+    if (workspace_bytes < need || (need && (!dev_workspace || off(dev_workspace, 4))))
+        return set_error(MTR_ERR_INVALID, "the workspace needs %lld bytes on 4, got %lld", (long long)need, (long long)workspace_bytes);
     DeviceGuard guard(device_id);
     if (!guard.ok) return set_error(MTR_ERR_HIP, "hipSetDevice(%d) failed", device_id);
     return launched("mtr_mx_matmul", mtr::launch_mx_matmul(dev_a_values, dev_a_scales, a_format, m, dev_b_values, dev_b_scales, n, d,
-                                                           dev_out, out_dtype, ld_out, static_cast<hipStream_t>(stream)));
+                                                           dev_out, out_dtype, ld_out, dev_workspace, static_cast<hipStream_t>(stream)));
 }
 
 int64_t mtr_token_logprobs_workspace(int64_t n, int64_t v, int32_t top_k) {

@@ -203,9 +203,13 @@ def mx_matmul(a: MxRows, b: MxRows, dtype=None, out=None):
         raise ValueError("out must be a (m, n) tensor of the dtype on the operands' GPU, its rows dense")
     if out.dtype not in (torch.float32, torch.bfloat16):
         raise TypeError(f"mx_matmul: unsupported dtype {out.dtype}")
-    _native.check(_native.lib().mtr_mx_matmul(
+    lib = _native.lib()
+    need = lib.mtr_mx_matmul_workspace(m, n, a.d)
+    workspace = torch.empty(need, dtype=torch.uint8, device=a.device) if need else None
+    _native.check(lib.mtr_mx_matmul(
         a.values.data_ptr(), a.scales.data_ptr(), FORMATS[a.format], m, b.values.data_ptr(), b.scales.data_ptr(), n, a.d,
-        out.data_ptr(), _code(out.dtype, "mx_matmul"), out.stride(0), a.device.index, _stream(a.device)))
+        out.data_ptr(), _code(out.dtype, "mx_matmul"), out.stride(0), workspace.data_ptr() if need else None, need, a.device.index,
+        _stream(a.device)))
     return out
 
 

@@ -109,8 +109,8 @@ def test_c_refusals_come_before_any_hip_call():
     refuses(norm(ldx=-8), "stride")
     assert norm(n=0) == _native.MTR_OK
 
-    def mm(av=at, af=1, m=2, bv=at, n=2, d=8, o=at, dt=0, ld=2):
-        return lib.mtr_mx_matmul(vp(av), vp(at), af, m, vp(bv), vp(at), n, d, vp(o), dt, ld, 0, None)
+    def mm(av=at, af=1, m=2, bv=at, n=2, d=8, o=at, dt=0, ld=2, w=None, wb=0):
+        return lib.mtr_mx_matmul(vp(av), vp(at), af, m, vp(bv), vp(at), n, d, vp(o), dt, ld, vp(w), wb, 0, None)
     refuses(mm(dt=3), "output dtype")
     refuses(mm(af=5), "format")
     refuses(mm(av=at + 4), "16 bytes")
@@ -118,6 +118,10 @@ def test_c_refusals_come_before_any_hip_call():
     refuses(mm(o=None), "NULL")
     refuses(mm(ld=1), "stride")
     refuses(mm(m=-1), "shape")
+    assert lib.mtr_mx_matmul_workspace(300, 500, 1000) > 0 and lib.mtr_mx_matmul_workspace(0, 5, 5) == 0
+    refuses(mm(m=300, n=500, d=1000, ld=500), "workspace")
+    refuses(mm(m=300, n=500, d=1000, ld=500, w=at, wb=64), "workspace")
+    refuses(mm(m=300, n=500, d=1000, ld=500, w=at + 2, wb=1 << 30), "workspace")
     assert mm(m=0, o=None) == _native.MTR_OK and mm(n=0, o=None) == _native.MTR_OK
 
     def lp(x=at, dt=0, n=2, v=100, ld=100, t=at, g=1, k=0, l=at, e=at, ti=at, tl=at, w=at, wb=1 << 20):
