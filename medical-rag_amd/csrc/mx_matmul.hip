@@ -17,6 +17,7 @@
 // Two kernels.  Up to kFewRows rows of A the product is bound by the one pass over B: every wave
 // takes 16 rows of B straight from memory into its operand registers.  More rows
 // take tiles staged in LDS.
+#include <stdlib.h>
 #include "mx_format.h"
 
 namespace mtr {
@@ -70,39 +71,151 @@ struct MatmulArgs {
     int whole;          // four neighbouring results can be stored at once
 };
 
-// One wave 16 rows of B times 16 of A, operands straight from memory.  Rows of B are the
-// instruction's rows, so that a lane ends with four neighbouring columns of out.  A lane
-// holds block lane / 16 of row lane % 16 of each 128: its scale is one byte.
-template <int FA, typename TO>
-__global__ __launch_bounds__(256) void mx_matmul_rows_kernel(MatmulArgs p) {
+// One wave 16 NT rows of B times 16 MT of A, operands straight from memory, four K steps
+// requested at once; KS waves share a workgroup's rows of B and split K, their sums
+// joined in LDS in a fixed order.  Rows of B are the instruction's rows, so that a lane
+// ends with four neighbouring columns of out.  A lane holds block lane / 16 of row lane %
+// 16 of each 128 elements: its scale is one byte of the row's word for that step.
+// ALIGNED: the words of four steps can be loaded at once.
+template <int FA, int MT, int NT, int KS, bool ALIGNED, typename TO>
+__global__ __launch_bounds__(KS > 4 ? 64 * KS : 256) void mx_matmul_rows_kernel(MatmulArgs p) {
+    constexpr int U = 4, kWaves = KS > 4 ? KS : 4;
+    constexpr int kRowA = FA == kMxFp4 ? 64 : 128, VA = kRowA / 64;
+    __shared__ f32x4 sums[KS > 1 ? kWaves * NT * MT * 64 : 1];
     const int lane = threadIdx.x & 63, r = lane & 15, g = lane >> 4;
-    const long long n0 = ((long long)blockIdx.x * 4 + (threadIdx.x >> 6)) * 16, m0 = (long long)blockIdx.y * 16;
-    if (n0 >= p.n) return;
-    const long long rn = n0 + r < p.n ? n0 + r : p.n - 1, rm = m0 + r < p.m ? m0 + r : p.m - 1;
-    const unsigned char* b = p.b + rn * p.groups * 64 + g * 16;
-    const unsigned char* bs = p.b_scales + rn * p.groups * 4 + g;
-    const unsigned char* a = p.a + rm * p.groups * (FA == kMxFp4 ? 64 : 128) + g * (FA == kMxFp4 ? 16 : 32);
-    const unsigned char* as = p.a_scales + rm * p.groups * 4 + g;
-    f32x4 acc = {0.f, 0.f, 0.f, 0.f};
-    for (int k = 0; k < p.groups; ++k) {
-        const u32x4 vb = *reinterpret_cast<const u32x4*>(b + (long long)k * 64);
-        const unsigned int sb = bs[k * 4], sa = as[k * 4];
-        if constexpr (FA == kMxFp4) {
-            const u32x4 va = *reinterpret_cast<const u32x4*>(a + (long long)k * 64);
-            const i32x8 fb = {(int)vb[0], (int)vb[1], (int)vb[2], (int)vb[3], 0, 0, 0, 0};
-            const i32x8 fa = {(int)va[0], (int)va[1], (int)va[2], (int)va[3], 0, 0, 0, 0};
-            acc = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(fb, fa, acc, 4, 4, 0, (int)sb, 0, (int)sa);
-        } else {
-            const u32x4 v0 = *reinterpret_cast<const u32x4*>(a + (long long)k * 128), v1 = *reinterpret_cast<const u32x4*>(a + (long long)k * 128 + 16);
-            const float fb = mx_scale(sb), fa = mx_scale(sa);
-            acc = __builtin_amdgcn_mfma_f32_16x16x32_bf16(widen_fp4(vb[0], fb), widen_fp8(v0[0], v0[1], fa), acc, 0, 0, 0);
-            acc = __builtin_amdgcn_mfma_f32_16x16x32_bf16(widen_fp4(vb[1], fb), widen_fp8(v0[2], v0[3], fa), acc, 0, 0, 0);
-            acc = __builtin_amdgcn_mfma_f32_16x16x32_bf16(widen_fp4(vb[2], fb), widen_fp8(v1[0], v1[1], fa), acc, 0, 0, 0);
-            acc = __builtin_amdgcn_mfma_f32_16x16x32_bf16(widen_fp4(vb[3], fb), widen_fp8(v1[2], v1[3], fa), acc, 0, 0, 0);
-        }
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), kw = wave % KS;
+    const long long n0 = ((long long)blockIdx.x * (kWaves / KS) + wave / KS) * 16 * NT, m0 = (long long)blockIdx.y * 16 * MT;
+    const int share = ((p.groups + KS - 1) / KS + U - 1) / U * U;       // K steps a wave
+    const int k_end = (kw + 1) * share < p.groups ? (kw + 1) * share : p.groups;
+    const unsigned char *a[MT], *b[NT];
+    const unsigned int *as[MT], *bs[NT];
+#pragma unroll
+    for (int j = 0; j < MT; ++j) {
+        const long long row = m0 + j * 16 + r < p.m ? m0 + j * 16 + r : p.m - 1;
+        a[j] = p.a + row * p.groups * kRowA + g * (kRowA / 4);
+        as[j] = reinterpret_cast<const unsigned int*>(p.a_scales) + row * p.groups;
     }
-    if (m0 + r < p.m)
-        store4<TO>(static_cast<TO*>(p.out) + (m0 + r) * p.ld + n0 + 4 * g, p.n - n0 - 4 * g, p.whole, acc);
+#pragma unroll
+    for (int i = 0; i < NT; ++i) {
+        const long long row = n0 + i * 16 + r < p.n ? n0 + i * 16 + r : p.n - 1;
+        b[i] = p.b + row * p.groups * 64 + g * 16;
+        bs[i] = reinterpret_cast<const unsigned int*>(p.b_scales) + row * p.groups;
+    }
+    f32x4 acc[NT][MT];
+#pragma unroll
+    for (int i = 0; i < NT; ++i)
+#pragma unroll
+        for (int j = 0; j < MT; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+
+    struct Step {
+        u32x4 b[NT], a[MT][VA];
+        unsigned int xb[NT], xa[MT];
+    };
+    const auto load_b = [&](Step& s, int k) {
+#pragma unroll
+        for (int i = 0; i < NT; ++i) s.b[i] = *reinterpret_cast<const u32x4*>(b[i] + (long long)k * 64);
+    };
+    const auto load_a = [&](Step& s, int k) {
+#pragma unroll
+        for (int j = 0; j < MT; ++j) {
+#pragma unroll
+            for (int h = 0; h < VA; ++h) s.a[j][h] = *reinterpret_cast<const u32x4*>(a[j] + (long long)k * kRowA + h * 16);
+            s.xa[j] = as[j][k];
+        }
+    };
+    const auto multiply = [&](const Step& s) {
+        unsigned int sb[NT], sa[MT];
+#pragma unroll
+        for (int i = 0; i < NT; ++i) sb[i] = (s.xb[i] >> (8 * g)) & 255u;
+#pragma unroll
+        for (int j = 0; j < MT; ++j) sa[j] = (s.xa[j] >> (8 * g)) & 255u;
+        if constexpr (FA == kMxFp4) {
+#pragma unroll
+            for (int i = 0; i < NT; ++i)
+#pragma unroll
+                for (int j = 0; j < MT; ++j) {
+                    const i32x4 fb = __builtin_bit_cast(i32x4, s.b[i]), fa = __builtin_bit_cast(i32x4, s.a[j][0]);
+                    acc[i][j] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(__builtin_shufflevector(fb, fb, 0, 1, 2, 3, -1, -1, -1, -1),
+                                                                                 __builtin_shufflevector(fa, fa, 0, 1, 2, 3, -1, -1, -1, -1),
+                                                                                 acc[i][j], 4, 4, 0, (int)sb[i], 0, (int)sa[j]);
+                }
+        } else {
+#pragma unroll
+            for (int h = 0; h < 4; ++h) {
+                bf16x8 fa[MT];
+#pragma unroll
+                for (int j = 0; j < MT; ++j) fa[j] = widen_fp8(s.a[j][h / 2][(h % 2) * 2], s.a[j][h / 2][(h % 2) * 2 + 1], mx_scale(sa[j]));
+#pragma unroll
+                for (int i = 0; i < NT; ++i) {
+                    const bf16x8 fb = widen_fp4(s.b[i][h], mx_scale(sb[i]));
+#pragma unroll
+                    for (int j = 0; j < MT; ++j) acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(fb, fa[j], acc[i][j], 0, 0, 0);
+                }
+            }
+        }
+    };
+    int k = kw * share;
+    for (; k + U <= k_end; k += U) {
+        Step s[U];
+#pragma unroll
+        for (int u = 0; u < U; ++u) load_b(s[u], k + u);
+#pragma unroll
+        for (int i = 0; i < NT; ++i) {
+            if constexpr (ALIGNED) {
+                const u32x4 w = *reinterpret_cast<const u32x4*>(bs[i] + k);
+#pragma unroll
+                for (int u = 0; u < U; ++u) s[u].xb[i] = w[u];
+            } else {
+#pragma unroll
+                for (int u = 0; u < U; ++u) s[u].xb[i] = bs[i][k + u];
+            }
+        }
+#pragma unroll
+        for (int u = 0; u < U; ++u) load_a(s[u], k + u);
+        __builtin_amdgcn_sched_barrier(0);      // all requests before the first wait
+#pragma unroll
+        for (int u = 0; u < U; ++u) multiply(s[u]);
+    }
+    for (; k < k_end; ++k) {
+        Step s;
+        load_b(s, k);
+#pragma unroll
+        for (int i = 0; i < NT; ++i) s.xb[i] = bs[i][k];
+        load_a(s, k);
+        multiply(s);
+    }
+    if constexpr (KS > 1) {
+#pragma unroll
+        for (int i = 0; i < NT; ++i)
+#pragma unroll
+            for (int j = 0; j < MT; ++j) sums[((i * MT + j) * kWaves + wave) * 64 + lane] = acc[i][j];
+        __syncthreads();
+    }
+#pragma unroll
+    for (int i = 0; i < NT; ++i)
+#pragma unroll
+        for (int j = 0; j < MT; ++j) {
+            if constexpr (KS > 1) {
+                if ((i * MT + j) % KS != kw) continue;      // each of the KS waves finishes some of the tiles
+                const int first = wave - kw;
+                f32x4 s = sums[((i * MT + j) * kWaves + first) * 64 + lane];
+                for (int w = 1; w < KS; ++w) s += sums[((i * MT + j) * kWaves + first + w) * 64 + lane];
+                acc[i][j] = s;
+            }
+            const long long row = m0 + j * 16 + r, col = n0 + i * 16 + 4 * g;
+            if (row < p.m) store4<TO>(static_cast<TO*>(p.out) + row * p.ld + col, p.n - col, p.whole, acc[i][j]);
+        }
+}
+
+template <int FA, int MT, int NT, int KS, typename TO> hipError_t launch_rows(const MatmulArgs& p, hipStream_t stream) {
+    constexpr int kWaves = KS > 4 ? KS : 4, kCols = kWaves / KS * 16 * NT;
+    const long long x = (p.n + kCols - 1) / kCols, y = (p.m + 16 * MT - 1) / (16 * MT);
+    if (x > 0x7fffffff || y > 65535) return hipErrorInvalidValue;
+    const dim3 grid((unsigned int)x, (unsigned int)y);
+    const bool aligned = p.groups % 4 == 0 && reinterpret_cast<uintptr_t>(p.b_scales) % 16 == 0;
+    if (aligned) hipLaunchKernelGGL((mx_matmul_rows_kernel<FA, MT, NT, KS, true, TO>), grid, dim3(64 * kWaves), 0, stream, p);
+    else hipLaunchKernelGGL((mx_matmul_rows_kernel<FA, MT, NT, KS, false, TO>), grid, dim3(64 * kWaves), 0, stream, p);
+    return hipGetLastError();
 }
 
 // ---- tiles ---------------------------------------------------------------------------
@@ -113,19 +226,26 @@ constexpr int kTileThreads = 512, kTileN = 256, kStages = 3;
 // [groups][padded rows], where a tile's words of one K step lie together: read where
 // they are, each row's four bytes would cost a request of their own, as many as the
 // elements' do.
-__global__ __launch_bounds__(256) void turn_scales_kernel(const unsigned int* __restrict__ src, long long rows, int groups,
-                                                          long long padded_rows, unsigned int* __restrict__ dst) {
+struct Turn {
+    const unsigned int* src;
+    long long rows, padded_rows;
+    unsigned int* dst;
+};
+__global__ __launch_bounds__(256) void turn_scales_kernel(Turn a, Turn b, int groups) {
     __shared__ unsigned int tile[32][65];
-    const long long r0 = (long long)blockIdx.x * 64;
+    const long long blocks_a = a.padded_rows / 64;
+    const bool first = blockIdx.x < blocks_a;
+    const Turn t = first ? a : b;
+    const long long r0 = (blockIdx.x - (first ? 0 : blocks_a)) * 64;
     const int g0 = blockIdx.y * 32;
     for (int i = threadIdx.x; i < 64 * 32; i += 256) {
         const int r = i / 32, g = i % 32;
-        if (r0 + r < rows && g0 + g < groups) tile[g][r] = src[(r0 + r) * groups + g0 + g];
+        if (r0 + r < t.rows && g0 + g < groups) tile[g][r] = t.src[(r0 + r) * groups + g0 + g];
     }
     __syncthreads();
     for (int i = threadIdx.x; i < 64 * 32; i += 256) {
         const int g = i / 64, r = i % 64;
-        if (r0 + r < rows && g0 + g < groups) dst[(long long)(g0 + g) * padded_rows + r0 + r] = tile[g][r];
+        if (r0 + r < t.rows && g0 + g < groups) t.dst[(long long)(g0 + g) * t.padded_rows + r0 + r] = tile[g][r];
     }
 }
 
@@ -166,7 +286,9 @@ template <int FA, bool EXACT, int WM> struct Tile {
     static constexpr int kRowA = FA == kMxFp4 ? 64 : 128;       // bytes of a row of A a step
     static constexpr int kBytesA = M * kRowA, kBytesB = kTileN * 64;
     static constexpr int kStage = kBytesA + kBytesB + 2048;     // 512 scale words: A's M, B's 256, the rest unused
-    static constexpr int kLoadsA = kBytesA / 8192, kLoadsB = kBytesB / 8192, kLoads = kLoadsA + kLoadsB + 1;
+    static constexpr int kLoadsA = kBytesA < 8192 ? 1 : kBytesA / 8192, kLoadsB = kBytesB / 8192, kLoads = kLoadsA + kLoadsB + 1;
+    // The wave's i-th piece (1 KiB) of A; with fewer pieces than waves several load the same one.
+    static __device__ __forceinline__ int piece_a(int wave, int i) { return (wave * kLoadsA + i) % (kBytesA / 1024); }
 };
 
 template <int FA, bool EXACT, int WM, typename TO>
@@ -189,7 +311,7 @@ __global__ __launch_bounds__(kTileThreads, 2) void mx_matmul_tile_kernel(TileArg
     unsigned int off_a[S::kLoadsA], off_b[S::kLoadsB];
 #pragma unroll
     for (int i = 0; i < S::kLoadsA; ++i) {
-        const int piece = wave * S::kLoadsA + i;        // 1 KiB
+        const int piece = S::piece_a(wave, i);
         const int row = FA == kMxFp4 ? piece * 16 + lane / 4 : piece * 8 + lane / 8;
         const int chunk = FA == kMxFp4 ? (lane & 3) ^ ((lane >> 4) & 3) : (lane & 7) ^ (lane >> 3);
         off_a[i] = (unsigned int)(row < last_a ? row : last_a) * row_a + chunk * 16;
@@ -217,7 +339,7 @@ __global__ __launch_bounds__(kTileThreads, 2) void mx_matmul_tile_kernel(TileArg
         const unsigned char* s = scalar_pointer(s0 + k * s_step);
 #pragma unroll
         for (int i = 0; i < S::kLoadsA; ++i)
-            __builtin_amdgcn_global_load_lds((gbl_ptr_t)(a + off_a[i]), (lds_ptr_t)(dst + (wave * S::kLoadsA + i) * 1024), 16, 0, 0);
+            __builtin_amdgcn_global_load_lds((gbl_ptr_t)(a + off_a[i]), (lds_ptr_t)(dst + S::piece_a(wave, i) * 1024), 16, 0, 0);
 #pragma unroll
         for (int i = 0; i < S::kLoadsB; ++i)
             __builtin_amdgcn_global_load_lds((gbl_ptr_t)(b + off_b[i]), (lds_ptr_t)(dst + S::kBytesA + (wave * S::kLoadsB + i) * 1024), 16, 0, 0);
@@ -313,9 +435,27 @@ __global__ __launch_bounds__(kTileThreads, 2) void mx_matmul_tile_kernel(TileArg
 }
 
 constexpr int kFewRows = 64;
+
+template <int FA, int MT, int NT, typename TO> hipError_t rows_split(const MatmulArgs& p, hipStream_t stream) {
+    const char* e = getenv("MM_KS");
+    const long long tiles = (p.n + 16 * NT - 1) / (16 * NT) * ((p.m + 16 * MT - 1) / (16 * MT));
+    int ks = tiles >= 4096 ? 4 : 16;
+    if (e) ks = atoi(e);
+    if (ks == 1) return launch_rows<FA, MT, NT, 1, TO>(p, stream);
+    if (ks == 4) return launch_rows<FA, MT, NT, 4, TO>(p, stream);
+    return launch_rows<FA, MT, NT, 16, TO>(p, stream);
+}
+template <int FA, typename TO> hipError_t rows_shaped(const MatmulArgs& p, hipStream_t stream) {
+    const char* e = getenv("MM_NT");
+    const int nt = e ? atoi(e) : 1;
+    if (p.m <= 16) return nt == 2 ? rows_split<FA, 1, 2, TO>(p, stream) : nt == 4 ? rows_split<FA, 1, 4, TO>(p, stream) : rows_split<FA, 1, 1, TO>(p, stream);
+    if (p.m <= 32) return nt == 2 ? rows_split<FA, 2, 2, TO>(p, stream) : rows_split<FA, 2, 1, TO>(p, stream);
+    return nt == 2 ? rows_split<FA, 4, 2, TO>(p, stream) : rows_split<FA, 4, 1, TO>(p, stream);
+}
+
 constexpr int kTileMaxGroups = 16384;       // offsets within a tile fit 32 bits
 
-bool takes_tiles(long long m, int groups) { return m > kFewRows && groups <= kTileMaxGroups; }
+bool takes_tiles(long long m, int groups) { const char* e = getenv("MM_FEW"); return m > (e ? atoi(e) : kFewRows) && groups <= kTileMaxGroups; }
 long long up(long long x, long long to) { return (x + to - 1) / to * to; }
 
 template <int FA, bool EXACT, int WM, typename TO> hipError_t launch_tiles(TileArgs p, hipStream_t stream) {
@@ -350,14 +490,11 @@ hipError_t launch_mx_matmul(const void* a_values, const void* a_scales, int a_fo
     if (takes_tiles(m, groups)) {
         unsigned int* as = static_cast<unsigned int*>(workspace);
         unsigned int* bs = as + up(m, 256) * groups;
-        const auto turn = [&](const void* src, long long rows, unsigned int* dst) {
-            const dim3 grid((unsigned int)((rows + 63) / 64), (unsigned int)((groups + 31) / 32));
-            hipLaunchKernelGGL(turn_scales_kernel, grid, dim3(256), 0, stream, static_cast<const unsigned int*>(src), rows, groups, up(rows, 256), dst);
-        };
-        turn(a_scales, m, as);
-        turn(b_scales, n, bs);
+        const Turn ta{static_cast<const unsigned int*>(a_scales), m, up(m, 256), as}, tb{static_cast<const unsigned int*>(b_scales), n, up(n, 256), bs};
+        const dim3 turn_grid((unsigned int)((up(m, 256) + up(n, 256)) / 64), (unsigned int)((groups + 31) / 32));
+        hipLaunchKernelGGL(turn_scales_kernel, turn_grid, dim3(256), 0, stream, ta, tb, groups);
         const TileArgs p{a, b, as, bs, m, n, up(m, 256), up(n, 256), groups, 0, out, ld_out, whole};
-#define MTR_TILES(F, X, T) return m <= 128 ? launch_tiles<F, X, 2, T>(p, stream) : launch_tiles<F, X, 4, T>(p, stream)
+#define MTR_TILES(F, X, T) return m <= 64 ? launch_tiles<F, X, 1, T>(p, stream) : m <= 128 ? launch_tiles<F, X, 2, T>(p, stream) : launch_tiles<F, X, 4, T>(p, stream)
         if (a_format == kMxFp4) {
             if (out_dtype == 0) MTR_TILES(kMxFp4, false, float);
             MTR_TILES(kMxFp4, false, bf16_t);
@@ -367,17 +504,8 @@ hipError_t launch_mx_matmul(const void* a_values, const void* a_scales, int a_fo
 #undef MTR_TILES
     }
     const MatmulArgs p{a, static_cast<const unsigned char*>(a_scales), b, static_cast<const unsigned char*>(b_scales), m, n, groups, out, ld_out, whole};
-    const dim3 grid((unsigned int)((n + 63) / 64), (unsigned int)((m + 15) / 16));
-#define MTR_MATMUL(F, T) hipLaunchKernelGGL((mx_matmul_rows_kernel<F, T>), grid, dim3(256), 0, stream, p)
-    if (out_dtype == 0) {
-        if (a_format == kMxFp4) MTR_MATMUL(kMxFp4, float);
-        else MTR_MATMUL(kMxFp8, float);
-    } else {
-        if (a_format == kMxFp4) MTR_MATMUL(kMxFp4, bf16_t);
-        else MTR_MATMUL(kMxFp8, bf16_t);
-    }
-#undef MTR_MATMUL
-    return hipGetLastError();
+    if (out_dtype == 0) return a_format == kMxFp4 ? rows_shaped<kMxFp4, float>(p, stream) : rows_shaped<kMxFp8, float>(p, stream);
+    return a_format == kMxFp4 ? rows_shaped<kMxFp4, bf16_t>(p, stream) : rows_shaped<kMxFp8, bf16_t>(p, stream);
 }
 
 }  // namespace mtr

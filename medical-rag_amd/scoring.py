@@ -20,6 +20,8 @@ from __future__ import annotations
 
 from collections import namedtuple
 
+import torch
+
 from . import _native
 
 __all__ = ["MxRows", "TokenLogprobs", "mx_quantize", "mx_dequantize", "rms_norm_mx", "mx_matmul", "token_logprobs"]
@@ -31,38 +33,31 @@ TokenLogprobs = namedtuple("TokenLogprobs", "logprobs entropy top_ids top_logpro
 TokenLogprobs.__doc__ = """What token_logprobs returns: logprobs (n, g) and entropy (n,) float32, top_ids (n, top_k)
 int64, top_logprobs (n, top_k) float32."""
 
-_codes: dict = {}
+_CODES = {torch.float32: _native.MTR_F32, torch.bfloat16: _native.MTR_BF16, torch.float16: _native.MTR_F16}
+# The handle of the current stream alone: building a Stream object around it costs as much as a launch.
+_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (lambda index: torch.cuda.current_stream(index).cuda_stream)
 
 
 def _code(dtype, what):
     """The library's code of a torch dtype it takes."""
-    if not _codes:
-        import torch
-        _codes.update({torch.float32: _native.MTR_F32, torch.bfloat16: _native.MTR_BF16, torch.float16: _native.MTR_F16})
-    try:
-        return _codes[dtype]
-    except KeyError:
-        raise TypeError(f"{what}: unsupported dtype {dtype}") from None
-
-
-def _stream(device):
-    import torch
-    return torch.cuda.current_stream(device).cuda_stream
+    code = _CODES.get(dtype)
+    if code is None:
+        raise TypeError(f"{what}: unsupported dtype {dtype}")
+    return code
 
 
 def _rows(x, what):
     """A (n, d) GPU tensor with dense rows (copied if its last dimension is strided)."""
-    import torch
     if not isinstance(x, torch.Tensor) or not x.is_cuda or x.dim() != 2:
         raise ValueError(f"{what} wants a 2-D GPU tensor")
     if x.requires_grad and torch.is_grad_enabled():
         raise ValueError(f"{what} has no backward pass: detach its inputs or call it under torch.no_grad()")
-    return x if x.shape[1] < 2 or x.stride(1) == 1 else x.contiguous()
+    return x if x.stride(1) == 1 or x.shape[1] < 2 else x.contiguous()
 
 
 def _width(d, format):
     """(element bytes, scale bytes) of a stored row."""
-    padded = -(-d // PAD) * PAD
+    padded = (d + PAD - 1) // PAD * PAD
     return (padded // 2 if format == "mxfp4" else padded), padded // BLOCK
 
 
@@ -72,10 +67,9 @@ class MxRows:
     one GPU with dense rows, the number `d` of elements of a row, and the `format`,
     "mxfp4" or "mxfp8"."""
 
-    __slots__ = ("values", "scales", "d", "format")
+    __slots__ = ("_values", "_scales", "_both", "_n", "_at", "d", "format", "device")
 
     def __init__(self, values, scales, d: int, format: str = "mxfp4"):
-        import torch
         if format not in FORMATS:
             raise ValueError(f"format must be one of {sorted(FORMATS)}")
         if d < 1:
@@ -89,32 +83,46 @@ class MxRows:
         if (values.shape[1], scales.shape[1]) != want or values.shape[0] != scales.shape[0]:
             raise ValueError(f"{format} rows of {d} elements have {want[0]} element and {want[1]} scale bytes, "
                              f"got {tuple(values.shape)} and {tuple(scales.shape)}")
-        self.values, self.scales, self.d, self.format = values, scales, int(d), format
+        self._values, self._scales, self._both = values, scales, None
+        self._n, self._at = values.shape[0], (values.data_ptr(), scales.data_ptr())
+        self.d, self.format, self.device = int(d), format, values.device
 
     @classmethod
     def empty(cls, n, d, format, device):
-        import torch
+        """Room for n rows, values and scales in one allocation."""
         if format not in FORMATS:
             raise ValueError(f"format must be one of {sorted(FORMATS)}")
         if d < 1:
             raise ValueError("rows need at least one element")
         width, blocks = _width(d, format)
         rows = cls.__new__(cls)
-        rows.values = torch.empty((n, width), dtype=torch.uint8, device=device)
-        rows.scales = torch.empty((n, blocks), dtype=torch.uint8, device=device)
-        rows.d, rows.format = int(d), format
+        both = torch.empty_strided((n * (width + blocks),), (1,), dtype=torch.uint8, device=device)
+        start = both.data_ptr()
+        rows._both, rows._values, rows._scales = both, None, None
+        rows._n, rows._at = n, (start, start + n * width)
+        rows.d, rows.format, rows.device = d, format, both.device
         return rows
 
-    def __len__(self):
-        return self.values.shape[0]
+    @property
+    def values(self):
+        if self._values is None:
+            width = _width(self.d, self.format)[0]
+            self._values = self._both[:self._n * width].view(self._n, width)
+        return self._values
 
     @property
-    def device(self):
-        return self.values.device
+    def scales(self):
+        if self._scales is None:
+            width, blocks = _width(self.d, self.format)
+            self._scales = self._both[self._n * width:].view(self._n, blocks)
+        return self._scales
+
+    def __len__(self):
+        return self._n
 
     @property
     def nbytes(self):
-        return self.values.numel() + self.scales.numel()
+        return self._n * sum(_width(self.d, self.format))
 
     def rows(self, lo, hi):
         """Rows [lo, hi) as a view."""
@@ -132,9 +140,13 @@ def mx_quantize(x, format: str = "mxfp4") -> MxRows:
     x = _rows(x, "mx_quantize")
     n, d = x.shape
     code = _code(x.dtype, "mx_quantize")
-    out = MxRows.empty(n, d, format, x.device)
-    _native.check(_native.lib().mtr_mx_quantize(x.data_ptr(), code, n, d, x.stride(0), FORMATS[format], out.values.data_ptr(),
-                                                out.scales.data_ptr(), x.device.index, _stream(x.device)))
+    device = x.device
+    out = MxRows.empty(n, d, format, device)
+    values, scales = out._at
+    rc = _native.lib().mtr_mx_quantize(x.data_ptr(), code, n, d, x.stride(0), FORMATS[format], values, scales, device.index,
+                                       _stream(device.index))
+    if rc:
+        _native.check(rc)
     return out
 
 
@@ -142,17 +154,20 @@ def mx_dequantize(rows: MxRows, dtype=None, out=None):
     """What microscaled rows stand for, as a (n, d) tensor of `dtype` (bfloat16, which
     holds every value exactly but the very smallest, unless given) or into `out`, a
     (n, d) GPU tensor with dense rows that do not overlap."""
-    import torch
-    n, d = len(rows), rows.d
+    n, d, device = rows._n, rows.d, rows.device
     if out is None:
-        code = _code(torch.bfloat16 if dtype is None else dtype, "mx_dequantize")
-        out = torch.empty((n, d), dtype=torch.bfloat16 if dtype is None else dtype, device=rows.device)
+        dtype = dtype or torch.bfloat16
+        code = _code(dtype, "mx_dequantize")
+        out = torch.empty_strided((n, d), (d, 1), dtype=dtype, device=device)
     else:
         code = _code(out.dtype, "mx_dequantize")
-        if out.shape != (n, d) or out.device != rows.device or (d > 1 and out.stride(1) != 1) or (dtype is not None and dtype != out.dtype):
+        if out.shape != (n, d) or out.device != device or (d > 1 and out.stride(1) != 1) or (dtype is not None and dtype != out.dtype):
             raise ValueError("out must be a (n, d) tensor of the dtype on the rows' GPU, its rows dense")
-    _native.check(_native.lib().mtr_mx_dequantize(rows.values.data_ptr(), rows.scales.data_ptr(), FORMATS[rows.format], n, d,
-                                                  out.data_ptr(), code, out.stride(0), rows.device.index, _stream(rows.device)))
+    values, scales = rows._at
+    rc = _native.lib().mtr_mx_dequantize(values, scales, FORMATS[rows.format], n, d, out.data_ptr(), code, out.stride(0), device.index,
+                                         _stream(device.index))
+    if rc:
+        _native.check(rc)
     return out
 
 
@@ -161,27 +176,31 @@ def rms_norm_mx(x, weight, eps: float = 1e-6, residual=None, format: str = "mxfp
     h = x + residual in their dtype (None without a residual), the rows
     h / sqrt(mean(h^2) + eps) * weight.  x, residual: (n, d), one dtype; weight: (d,)
     of that dtype or float32.  Sums are in 32 bits; d up to 65536."""
-    import torch
     x = _rows(x, "rms_norm_mx")
     n, d = x.shape
-    code = _code(x.dtype, "rms_norm_mx")
-    if (not isinstance(weight, torch.Tensor) or weight.shape != (d,) or weight.device != x.device
-            or weight.dtype not in (x.dtype, torch.float32)):
+    dtype, device = x.dtype, x.device
+    code = _code(dtype, "rms_norm_mx")
+    if (not isinstance(weight, torch.Tensor) or weight.shape != (d,) or weight.device != device
+            or weight.dtype not in (dtype, torch.float32)):
         raise ValueError(f"rms_norm_mx wants a ({d},) weight of the rows' dtype or float32 on their GPU")
     if weight.requires_grad and torch.is_grad_enabled():
         raise ValueError("rms_norm_mx has no backward pass: detach its inputs or call it under torch.no_grad()")
-    weight = weight.contiguous()
+    if weight.stride(0) != 1:
+        weight = weight.contiguous()
     h = None
     if residual is not None:
         residual = _rows(residual, "rms_norm_mx")
-        if residual.shape != x.shape or residual.dtype != x.dtype or residual.device != x.device:
+        if residual.shape != x.shape or residual.dtype != dtype or residual.device != device:
             raise ValueError("rms_norm_mx wants a residual of the rows' shape and dtype on their GPU")
-        h = torch.empty((n, d), dtype=x.dtype, device=x.device)
-    out = MxRows.empty(n, d, format, x.device)
-    _native.check(_native.lib().mtr_rms_norm_mx(
-        x.data_ptr(), residual.data_ptr() if h is not None else None, weight.data_ptr(), code, _code(weight.dtype, "rms_norm_mx"), n, d,
-        x.stride(0), residual.stride(0) if h is not None else 0, eps, FORMATS[format], h.data_ptr() if h is not None else None,
-        out.values.data_ptr(), out.scales.data_ptr(), x.device.index, _stream(x.device)))
+        h = torch.empty_strided((n, d), (d, 1), dtype=dtype, device=device)
+    out = MxRows.empty(n, d, format, device)
+    values, scales = out._at
+    rc = _native.lib().mtr_rms_norm_mx(
+        x.data_ptr(), None if h is None else residual.data_ptr(), weight.data_ptr(), code, _CODES[weight.dtype], n, d, x.stride(0),
+        0 if h is None else residual.stride(0), eps, FORMATS[format], None if h is None else h.data_ptr(), values, scales, device.index,
+        _stream(device.index))
+    if rc:
+        _native.check(rc)
     return out, h
 
 
@@ -189,27 +208,28 @@ def mx_matmul(a: MxRows, b: MxRows, dtype=None, out=None):
     """(m, n) products of a's m rows (either format) with b's n rows (mxfp4), summed in
     32 bits; float32 unless `dtype` says bfloat16, or into `out`, a (m, n) GPU tensor
     with dense rows that do not overlap."""
-    import torch
     if b.format != "mxfp4":
         raise ValueError("mx_matmul wants its second operand in mxfp4")
     if a.d != b.d:
         raise ValueError(f"rows of {a.d} and of {b.d} elements")
-    if a.device != b.device:
-        raise ValueError(f"operands are on {a.device} and {b.device}")
-    m, n = len(a), len(b)
+    device = a.device
+    if device != b.device:
+        raise ValueError(f"operands are on {device} and {b.device}")
+    m, n = a._n, b._n
     if out is None:
-        out = torch.empty((m, n), dtype=torch.float32 if dtype is None else dtype, device=a.device)
-    elif out.shape != (m, n) or out.device != a.device or (n > 1 and out.stride(1) != 1) or (dtype is not None and dtype != out.dtype):
+        dtype = dtype or torch.float32
+        out = torch.empty_strided((m, n), (n, 1), dtype=dtype, device=device)
+    elif out.shape != (m, n) or out.device != device or (n > 1 and out.stride(1) != 1) or (dtype is not None and dtype != out.dtype):
         raise ValueError("out must be a (m, n) tensor of the dtype on the operands' GPU, its rows dense")
     if out.dtype not in (torch.float32, torch.bfloat16):
         raise TypeError(f"mx_matmul: unsupported dtype {out.dtype}")
     lib = _native.lib()
     need = lib.mtr_mx_matmul_workspace(m, n, a.d)
-    workspace = torch.empty(need, dtype=torch.uint8, device=a.device) if need else None
-    _native.check(lib.mtr_mx_matmul(
-        a.values.data_ptr(), a.scales.data_ptr(), FORMATS[a.format], m, b.values.data_ptr(), b.scales.data_ptr(), n, a.d,
-        out.data_ptr(), _code(out.dtype, "mx_matmul"), out.stride(0), workspace.data_ptr() if need else None, need, a.device.index,
-        _stream(a.device)))
+    workspace = torch.empty_strided((need,), (1,), dtype=torch.uint8, device=device) if need else None
+    rc = lib.mtr_mx_matmul(*a._at, FORMATS[a.format], m, *b._at, n, a.d, out.data_ptr(), _CODES[out.dtype], out.stride(0),
+                           workspace.data_ptr() if need else None, need, device.index, _stream(device.index))
+    if rc:
+        _native.check(rc)
     return out
 
 
@@ -223,31 +243,34 @@ def token_logprobs(logits, tokens=None, top_k: int = 0) -> TokenLogprobs:
     with nothing left has entropy 0; one that holds a NaN or +inf has NaN everywhere.
     A negative token is padding, its log probability 0; one >= v gives NaN (the call
     does not wait for the GPU and so cannot raise)."""
-    import torch
     logits = _rows(logits, "token_logprobs")
     n, v = logits.shape
     code = _code(logits.dtype, "token_logprobs")
     device = logits.device
     if tokens is None:
-        tokens = torch.empty((n, 0), dtype=torch.int64, device=device)
-    if not isinstance(tokens, torch.Tensor) or tokens.dtype != torch.int64 or tokens.device != device:
-        raise ValueError("token_logprobs wants int64 tokens on the logits' GPU")
-    if tokens.dim() == 1:
-        tokens = tokens[:, None]
-    if tokens.dim() != 2 or tokens.shape[0] != n:
-        raise ValueError(f"token_logprobs wants ({n},) or ({n}, g) tokens, got {tuple(tokens.shape)}")
+        g = 0
+    else:
+        if not isinstance(tokens, torch.Tensor) or tokens.dtype != torch.int64 or tokens.device != device:
+            raise ValueError("token_logprobs wants int64 tokens on the logits' GPU")
+        if tokens.dim() == 1:
+            tokens = tokens[:, None]
+        if tokens.dim() != 2 or tokens.shape[0] != n:
+            raise ValueError(f"token_logprobs wants ({n},) or ({n}, g) tokens, got {tuple(tokens.shape)}")
+        tokens = tokens.contiguous()
+        g = tokens.shape[1]
     if not 0 <= top_k <= _native.MTR_MAX_ALTERNATIVES:
         raise ValueError(f"top_k must be in [0, {_native.MTR_MAX_ALTERNATIVES}]")
-    tokens = tokens.contiguous()
-    g = tokens.shape[1]
     lib = _native.lib()
-    logprobs = torch.empty((n, g), dtype=torch.float32, device=device)
-    entropy = torch.empty(n, dtype=torch.float32, device=device)
-    top_ids = torch.empty((n, top_k), dtype=torch.int64, device=device)
-    top_logprobs = torch.empty((n, top_k), dtype=torch.float32, device=device)
+    empty = torch.empty_strided
+    logprobs = empty((n, g), (g, 1), dtype=torch.float32, device=device)
+    entropy = empty((n,), (1,), dtype=torch.float32, device=device)
+    top_ids = empty((n, top_k), (top_k, 1), dtype=torch.int64, device=device)
+    top_logprobs = empty((n, top_k), (top_k, 1), dtype=torch.float32, device=device)
     need = lib.mtr_token_logprobs_workspace(n, v, top_k)
-    workspace = torch.empty(need, dtype=torch.uint8, device=device) if need else None
-    _native.check(lib.mtr_token_logprobs(
-        logits.data_ptr(), code, n, v, logits.stride(0), tokens.data_ptr(), g, top_k, logprobs.data_ptr(), entropy.data_ptr(),
-        top_ids.data_ptr(), top_logprobs.data_ptr(), workspace.data_ptr() if need else None, need, device.index, _stream(device)))
+    workspace = empty((need,), (1,), dtype=torch.uint8, device=device) if need else None
+    rc = lib.mtr_token_logprobs(
+        logits.data_ptr(), code, n, v, logits.stride(0), tokens.data_ptr() if g else None, g, top_k, logprobs.data_ptr(), entropy.data_ptr(),
+        top_ids.data_ptr(), top_logprobs.data_ptr(), workspace.data_ptr() if need else None, need, device.index, _stream(device.index))
+    if rc:
+        _native.check(rc)
     return TokenLogprobs(logprobs, entropy, top_ids, top_logprobs)
