@@ -14,10 +14,9 @@
 // where they are rounded to bfloat16, whose half step of 4e-3 is a hundred times the
 // difference.
 //
-// Two kernels.  Up to kFewRows rows of A the product is bound by the one pass over B: every wave
-// takes 16 rows of B straight from memory into its operand registers.  More rows
-// take tiles staged in LDS.
-#include <stdlib.h>
+// Two kernels.  Few rows of A, or few of both, are bound by the one pass over B or by
+// how many waves there are: every wave takes its rows of B straight from memory into
+// its operand registers.  Larger products take tiles staged in LDS.
 #include "mx_format.h"
 
 namespace mtr {
@@ -221,6 +220,7 @@ template <int FA, int MT, int NT, int KS, typename TO> hipError_t launch_rows(co
 // ---- tiles ---------------------------------------------------------------------------
 
 constexpr int kTileThreads = 512, kTileN = 256, kStages = 3;
+constexpr int kTileMaxGroups = 16384;       // offsets within a tile fit 32 bits
 
 // Scale words (the four scale bytes of 128 elements) turned from [rows][groups] to
 // [groups][padded rows], where a tile's words of one K step lie together: read where
@@ -421,41 +421,65 @@ __global__ __launch_bounds__(kTileThreads, 2) void mx_matmul_tile_kernel(TileArg
         }
     }
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");    // the loads past the last step still write to this workgroup's LDS
+    // The results leave through LDS, 16 rows of A's a round, so that a store covers whole rows of the
+    // wave's columns: straight from the accumulators it would touch 16 rows, 4 columns each.
+    barrier_keeping_loads();
+    constexpr int NW = S::NT * 16, kPitch = NW + 4;     // 4 words on: 16 rows start in different banks
+    float* mine = reinterpret_cast<float*>(smem) + wave * 16 * kPitch;
+    const long long left = p.n - (n0 + wn * NW);        // columns that exist
 #pragma unroll
     for (int j = 0; j < S::MT; ++j) {
-        const long long row = m0 + wm * 64 + j * 16 + r;
-        if (row >= p.m) continue;
-        TO* o = static_cast<TO*>(p.out) + row * p.ld;
 #pragma unroll
-        for (int i = 0; i < S::NT; ++i) {
-            const long long col = n0 + (wn * S::NT + i) * 16 + 4 * g;
-            store4<TO>(o + col, p.n - col, p.whole, acc[i][j]);
+        for (int i = 0; i < S::NT; ++i) *reinterpret_cast<f32x4*>(mine + r * kPitch + i * 16 + 4 * g) = acc[i][j];
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+        const long long row0 = m0 + wm * 64 + j * 16;
+        TO* o = static_cast<TO*>(p.out) + row0 * p.ld + n0 + wn * NW;
+        if (p.whole) {
+            constexpr int kLanes = NW / 4, kRows = 64 / kLanes;     // lanes a row, rows a store
+#pragma unroll
+            for (int s = 0; s < 16 / kRows; ++s) {
+                const int row = s * kRows + lane / kLanes, col = lane % kLanes * 4;
+                const f32x4 v = *reinterpret_cast<const f32x4*>(mine + row * kPitch + col);
+                if (row0 + row < p.m) store4<TO>(o + row * p.ld + col, left - col, true, v);
+            }
+        } else {
+            constexpr int kLanes = NW < 64 ? NW : 64, kRows = 64 / kLanes;
+#pragma unroll 4
+            for (int s = 0; s < 16 / kRows; ++s) {
+                const int row = s * kRows + lane / kLanes;
+                if (row0 + row < p.m)
+#pragma unroll
+                    for (int c = 0; c < NW; c += kLanes) {
+                        const int col = c + lane % kLanes;
+                        if (col < left) o[row * p.ld + col] = from_f32<TO>(mine[row * kPitch + col]);
+                    }
+            }
         }
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
     }
 }
 
-constexpr int kFewRows = 64;
 
-template <int FA, int MT, int NT, typename TO> hipError_t rows_split(const MatmulArgs& p, hipStream_t stream) {
-    const char* e = getenv("MM_KS");
-    const long long tiles = (p.n + 16 * NT - 1) / (16 * NT) * ((p.m + 16 * MT - 1) / (16 * MT));
-    int ks = tiles >= 4096 ? 4 : 16;
-    if (e) ks = atoi(e);
-    if (ks == 1) return launch_rows<FA, MT, NT, 1, TO>(p, stream);
-    if (ks == 4) return launch_rows<FA, MT, NT, 4, TO>(p, stream);
-    return launch_rows<FA, MT, NT, 16, TO>(p, stream);
+// Tiles fill the chip from about 48 of them on; below, and for rows too long for their 32-bit offsets, every wave
+// on its own is faster (measured, k = 4096, 8 bits to fp32, microseconds, tiles / waves: 32 x 131072 96 / 109,
+// 16 x 131072 91 / 76, 256 x 16384 99 / 88, 512 x 16384 101 / 172, 512 x 4032 97 / 46, 1024 x 4032 100 / 88).
+bool takes_tiles(long long m, long long n, int groups) { return m * n > 3000000 && groups <= kTileMaxGroups; }
+
+template <int FA, int MT, typename TO> hipError_t rows_split(const MatmulArgs& p, hipStream_t stream) {
+    // 16 rows of B a wave while that gives no CU a second workgroup, else 32; K split over four waves until there are
+    // waves enough without (measured, k = 4096, 8 bits, microseconds: 64 x 4032 12.5 with 16 rows / 14.2 with 32,
+    // 128 x 4032 22 / 15; 256 x 4032 29.6 split / 44.8 not, 512 x 4032 55.5 / 46.3, 16 x 131072 81 / 76).
+    const long long m_tiles = (p.m + 16 * MT - 1) / (16 * MT), narrow = m_tiles * ((p.n + 15) / 16);
+    if (narrow <= 256) return launch_rows<FA, MT, 1, 4, TO>(p, stream);
+    if (narrow / 2 < (MT == 1 ? 4000 : 1000)) return launch_rows<FA, MT, 2, 4, TO>(p, stream);
+    return launch_rows<FA, MT, 2, 1, TO>(p, stream);
 }
 template <int FA, typename TO> hipError_t rows_shaped(const MatmulArgs& p, hipStream_t stream) {
-    const char* e = getenv("MM_NT");
-    const int nt = e ? atoi(e) : 1;
-    if (p.m <= 16) return nt == 2 ? rows_split<FA, 1, 2, TO>(p, stream) : nt == 4 ? rows_split<FA, 1, 4, TO>(p, stream) : rows_split<FA, 1, 1, TO>(p, stream);
-    if (p.m <= 32) return nt == 2 ? rows_split<FA, 2, 2, TO>(p, stream) : rows_split<FA, 2, 1, TO>(p, stream);
-    return nt == 2 ? rows_split<FA, 4, 2, TO>(p, stream) : rows_split<FA, 4, 1, TO>(p, stream);
+    if (p.m <= 16) return rows_split<FA, 1, TO>(p, stream);
+    if (p.m <= 32) return rows_split<FA, 2, TO>(p, stream);
+    return rows_split<FA, 4, TO>(p, stream);
 }
 
-constexpr int kTileMaxGroups = 16384;       // offsets within a tile fit 32 bits
-
-bool takes_tiles(long long m, int groups) { const char* e = getenv("MM_FEW"); return m > (e ? atoi(e) : kFewRows) && groups <= kTileMaxGroups; }
 long long up(long long x, long long to) { return (x + to - 1) / to * to; }
 
 template <int FA, bool EXACT, int WM, typename TO> hipError_t launch_tiles(TileArgs p, hipStream_t stream) {
@@ -476,7 +500,7 @@ template <int FA, bool EXACT, int WM, typename TO> hipError_t launch_tiles(TileA
 
 long long mx_matmul_workspace(long long m, long long n, int d) {
     const int groups = mx_padded(d) / 128;
-    return takes_tiles(m, groups) ? (up(m, 256) + up(n, 256)) * groups * 4 : 0;
+    return takes_tiles(m, n, groups) ? (up(m, 256) + up(n, 256)) * groups * 4 : 0;
 }
 
 hipError_t launch_mx_matmul(const void* a_values, const void* a_scales, int a_format, long long m, const void* b_values,
@@ -487,7 +511,7 @@ hipError_t launch_mx_matmul(const void* a_values, const void* a_scales, int a_fo
     const int whole = ld_out % 4 == 0 && reinterpret_cast<uintptr_t>(out) % (4 * size) == 0;
     const auto* a = static_cast<const unsigned char*>(a_values);
     const auto* b = static_cast<const unsigned char*>(b_values);
-    if (takes_tiles(m, groups)) {
+    if (takes_tiles(m, n, groups)) {
         unsigned int* as = static_cast<unsigned int*>(workspace);
         unsigned int* bs = as + up(m, 256) * groups;
         const Turn ta{static_cast<const unsigned int*>(a_scales), m, up(m, 256), as}, tb{static_cast<const unsigned int*>(b_scales), n, up(n, 256), bs};
