@@ -284,7 +284,8 @@ __device__ __forceinline__ const unsigned char* scalar_pointer(const unsigned ch
 
 // s_barrier without the drain of outstanding loads that __syncthreads() adds.
 __device__ __forceinline__ void barrier_keeping_loads() {
-    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+    asm volatile("" ::: "memory");
+    __builtin_amdgcn_s_waitcnt(0xC07F);     // lgkmcnt(0), as the builtin: the compiler then knows that no LDS read is left to wait for
     __builtin_amdgcn_s_barrier();
     asm volatile("" ::: "memory");
 }
@@ -302,9 +303,10 @@ template <int FA> __device__ __forceinline__ f32x4 scaled_mfma(const i32x8& fb, 
 
 // A tile of 64 WM rows of A times 256 rows of B; eight waves, WM x (8 / WM), each 64 rows
 // of A times 32 WM of B.  K steps of 128 elements in a ring of three LDS stages, filled
-// by 16-byte direct-to-LDS loads two steps ahead; one barrier a step.  A wave waits for its
-// own loads of step s (all but the newest step's), the barrier then says that everybody's
-// have landed, and that everybody is done with step s - 1, whose stage step s + 2 takes.
+// by 16-byte direct-to-LDS loads two steps or more ahead; one barrier a step.  A wave waits
+// for its own loads of a step (all but the newest step's), the barrier then says that
+// everybody's have landed, and that everybody is done with the stage that the next
+// loads go to.
 // 16-byte chunks are swizzled on the loads' source addresses: LDS serves a 16-byte read
 // in four parts of 16 lanes, {0-3, 12-15, 20-27}, {4-11, 16-19, 28-31} and the same
 // 32 lanes on (measured), from 64 banks; with the row's low three bits (rows of 128
@@ -385,69 +387,117 @@ __global__ __launch_bounds__(kTileThreads, 2) void mx_matmul_tile_kernel(TileArg
 #pragma unroll
         for (int j = 0; j < S::MT; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
 
-#pragma unroll
-    for (int i = 0; i < S::kLoads; ++i) request(i, 0, smem);
-#pragma unroll
-    for (int i = 0; i < S::kLoads; ++i) request(i, p.groups > 1 ? 1 : 0, smem + S::kStage);
-    int now = 0;
-    for (int k = 0; k < p.groups; ++k) {
-        asm volatile("s_waitcnt vmcnt(%0)" ::"n"(S::kLoads) : "memory");
-        barrier_keeping_loads();
-        const int k2 = k + 2 < p.groups ? k + 2 : p.groups - 1;
-        unsigned char* next = smem + (now == 0 ? 2 : now - 1) * S::kStage;     // (now + 2) % 3
-        const unsigned char* st = smem + now * S::kStage;
-        now = now == 2 ? 0 : now + 1;
-        const unsigned char* sa = st + wm * 64 * S::kRowA;
-        const unsigned char* sb = st + S::kBytesA + wn * S::NT * 16 * 64;
+    const auto step_at = [&](int k) { return k < p.groups ? k : p.groups - 1; };     // loads past the last step fetch it again
+    constexpr int kWords = (S::NT + 3) / 4;
+    const auto read_words = [&](const unsigned char* st, unsigned int& xa, unsigned int (&xb)[kWords]) {
         const unsigned int* words = reinterpret_cast<const unsigned int*>(st + S::kBytesA + S::kBytesB);
-        const unsigned int xa = words[wm * 64 + lane];
+        xa = words[wm * 64 + lane];
         // a wave's columns are whole groups of 64 rows of B, or the half group that a wave of the narrowest form has
-        unsigned int xb[(S::NT + 3) / 4];
 #pragma unroll
-        for (int i = 0; i < (S::NT + 3) / 4; ++i) xb[i] = words[S::M + (wn * S::NT / 4 + i) * 64 + lane] >> (S::NT < 4 ? wn % 2 * 16 : 0);
-        // The loads of step k + 2 go out one by one between the multiplications: a load holds its wave up for 100 to 200
-        // cycles, and the reads of LDS two operands ahead.  The order is pinned; left to itself the compiler has all
-        // loads first and the matrix cores idle meanwhile.
-        if constexpr (!EXACT) {
-            i32x8 fa[S::MT];
-#pragma unroll
-            for (int j = 0; j < S::MT; ++j) {
-                const unsigned char* row = sa + (j * 16 + r) * S::kRowA;
-                if constexpr (FA == kMxFp4) {
-                    const i32x4 v = *reinterpret_cast<const i32x4*>(row + ((g ^ ((r >> 1) & 3)) << 4));
-                    fa[j] = __builtin_shufflevector(v, v, 0, 1, 2, 3, -1, -1, -1, -1);
-                } else {        // the instruction takes elements 16 g .. and 64 + 16 g .. of an 8-bit row
-                    const i32x4 v = *reinterpret_cast<const i32x4*>(row + ((g ^ (r & 7)) << 4));
-                    const i32x4 w = *reinterpret_cast<const i32x4*>(row + (((4 + g) ^ (r & 7)) << 4));
-                    fa[j] = __builtin_shufflevector(v, w, 0, 1, 2, 3, 4, 5, 6, 7);
-                }
+        for (int i = 0; i < kWords; ++i) xb[i] = words[S::M + (wn * S::NT / 4 + i) * 64 + lane] >> (S::NT < 4 ? wn % 2 * 16 : 0);
+    };
+    if constexpr (!EXACT) {
+        i32x8 fa[S::MT];
+        i32x4 fb[S::NT];
+        const auto read_a = [&](const unsigned char* st, int j) {
+            const unsigned char* row = st + (wm * 64 + j * 16 + r) * S::kRowA;
+            if constexpr (FA == kMxFp4) {
+                const i32x4 v = *reinterpret_cast<const i32x4*>(row + ((g ^ ((r >> 1) & 3)) << 4));
+                fa[j] = __builtin_shufflevector(v, v, 0, 1, 2, 3, -1, -1, -1, -1);
+            } else {        // the instruction takes elements 16 g .. and 64 + 16 g .. of an 8-bit row
+                const i32x4 v = *reinterpret_cast<const i32x4*>(row + ((g ^ (r & 7)) << 4));
+                const i32x4 w = *reinterpret_cast<const i32x4*>(row + (((4 + g) ^ (r & 7)) << 4));
+                fa[j] = __builtin_shufflevector(v, w, 0, 1, 2, 3, 4, 5, 6, 7);
             }
-            i32x4 fb[S::NT];
+        };
+        const auto read_b = [&](const unsigned char* st, int i) {
+            fb[i] = *reinterpret_cast<const i32x4*>(st + S::kBytesA + ((wn * S::NT + i) * 16 + r) * 64 + ((g ^ ((r >> 1) & 3)) << 4));
+        };
+        constexpr int H = S::NT / 2, kReadsA = FA == kMxFp4 ? 1 : 2, kPer = (S::kLoads + S::MT - 1) / S::MT;
 #pragma unroll
-            for (int i = 0; i < S::NT; ++i) fb[i] = *reinterpret_cast<const i32x4*>(sb + (i * 16 + r) * 64 + ((g ^ ((r >> 1) & 3)) << 4));
+        for (int s = 0; s < 3; ++s)
 #pragma unroll
-            for (int l = 0; l < S::kLoads; ++l) request(l, k2, next);
+            for (int i = 0; i < S::kLoads; ++i) request(i, step_at(s), smem + s * S::kStage);
+        asm volatile("s_waitcnt vmcnt(%0)" ::"n"(2 * S::kLoads) : "memory");
+        barrier_keeping_loads();
+        unsigned int xa, xb[kWords];
+        read_words(smem, xa, xb);
 #pragma unroll
-            for (int i = 0; i < S::NT; ++i)
+        for (int j = 0; j < S::MT; ++j) read_a(smem, j);
+#pragma unroll
+        for (int i = 0; i < H; ++i) read_b(smem, i);
+        int now = 0;
+        for (int k = 0; k < p.groups; ++k) {
+            unsigned char* st = smem + now * S::kStage;
+            now = now == 2 ? 0 : now + 1;
+            const unsigned char* st1 = smem + now * S::kStage;
+            // first half: the second half's operands of B come in
+#pragma unroll
+            for (int i = H; i < S::NT; ++i) read_b(st, i);
+#pragma unroll
+            for (int i = 0; i < H; ++i)
 #pragma unroll
                 for (int j = 0; j < S::MT; ++j)
                     acc[i][j] = scaled_mfma<FA>(__builtin_shufflevector(fb[i], fb[i], 0, 1, 2, 3, -1, -1, -1, -1), fa[j], acc[i][j], xb[i / 4],
                                                 i % 4, xa, j);
-            constexpr int kWords = 1 + (S::NT + 3) / 4, kFirst = S::NT < 2 ? S::NT : 2, kPer = (S::NT - kFirst + 1) / 2;
-            constexpr int kGroups = S::NT * S::MT - 2 * S::MT, kEvery = kGroups / S::kLoads > 0 ? kGroups / S::kLoads : 1;
-            __builtin_amdgcn_sched_group_barrier(0x100, kWords + S::MT * (FA == kMxFp4 ? 1 : 2) + kFirst, 0);
-            if constexpr (S::NT > 2) {
-                __builtin_amdgcn_sched_group_barrier(0x008, S::MT, 0);
-                __builtin_amdgcn_sched_group_barrier(0x100, kPer, 0);
-                __builtin_amdgcn_sched_group_barrier(0x008, S::MT, 0);
-                __builtin_amdgcn_sched_group_barrier(0x100, S::NT - kFirst - kPer, 0);
+#pragma unroll
+            for (int i = 0; i < H; ++i) {
+                __builtin_amdgcn_sched_group_barrier(0x008, S::MT / 2, 0);
+                __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
+                __builtin_amdgcn_sched_group_barrier(0x008, S::MT / 2, 0);
+            }
+            // Everybody is done reading step k, and step k + 1 has landed for everybody.
+            asm volatile("s_waitcnt vmcnt(%0)" ::"n"(S::kLoads) : "memory");
+            barrier_keeping_loads();
+            // second half, A's operands outside: each is replaced by the next step's as soon as it is used up, B's first
+            // half too, and the loads of step k + 3 go out between (one holds its wave up for 100 to 200 cycles)
+            unsigned int ya, yb[kWords];
+            read_words(st1, ya, yb);
+#pragma unroll
+            for (int j = 0; j < S::MT; ++j) {
+#pragma unroll
+                for (int i = H; i < S::NT; ++i)
+                    acc[i][j] = scaled_mfma<FA>(__builtin_shufflevector(fb[i], fb[i], 0, 1, 2, 3, -1, -1, -1, -1), fa[j], acc[i][j], xb[i / 4],
+                                                i % 4, xa, j);
+                read_a(st1, j);
+                if (j < H) read_b(st1, j);
+#pragma unroll
+                for (int l = j * kPer; l < (j + 1) * kPer && l < S::kLoads; ++l) request(l, step_at(k + 3), st);
+            }
+            __builtin_amdgcn_sched_group_barrier(0x100, 1 + kWords, 0);
+#pragma unroll
+            for (int j = 0; j < H; ++j) {
+                __builtin_amdgcn_sched_group_barrier(0x008, S::NT - H, 0);
+                __builtin_amdgcn_sched_group_barrier(0x100, kReadsA + 1, 0);
+                __builtin_amdgcn_sched_group_barrier(0x020, kPer, 0);
             }
 #pragma unroll
-            for (int l = 0; l < S::kLoads; ++l) {
-                __builtin_amdgcn_sched_group_barrier(0x020, 1, 0);
-                __builtin_amdgcn_sched_group_barrier(0x008, kEvery, 0);
+            for (int j = H; j < S::MT; ++j) {
+                __builtin_amdgcn_sched_group_barrier(0x008, S::NT - H, 0);
+                __builtin_amdgcn_sched_group_barrier(0x100, kReadsA, 0);
+                __builtin_amdgcn_sched_group_barrier(0x020, kPer, 0);
             }
-        } else {
+            xa = ya;
+#pragma unroll
+            for (int i = 0; i < kWords; ++i) xb[i] = yb[i];
+        }
+    } else {
+#pragma unroll
+        for (int s = 0; s < 2; ++s)
+#pragma unroll
+            for (int i = 0; i < S::kLoads; ++i) request(i, step_at(s), smem + s * S::kStage);
+        int now = 0;
+        for (int k = 0; k < p.groups; ++k) {
+            asm volatile("s_waitcnt vmcnt(%0)" ::"n"(S::kLoads) : "memory");
+            barrier_keeping_loads();
+            const int k2 = step_at(k + 2);
+            unsigned char* next = smem + (now == 0 ? 2 : now - 1) * S::kStage;     // (now + 2) % 3
+            const unsigned char* st = smem + now * S::kStage;
+            now = now == 2 ? 0 : now + 1;
+            const unsigned char* sa = st + wm * 64 * S::kRowA;
+            const unsigned char* sb = st + S::kBytesA + wn * S::NT * 16 * 64;
+            unsigned int xa, xb[kWords];
+            read_words(st, xa, xb);
             // elements 32 g .. of both, eight at a time; A's next eight are read while these are multiplied
             u32x4 vb[S::NT];
             unsigned int va[2][S::MT][2];
