@@ -222,7 +222,7 @@ template <int FA, int MT, int NT, int KS, typename TO> hipError_t launch_rows(co
 
 // ---- tiles ---------------------------------------------------------------------------
 
-constexpr int kTileThreads = 512, kTileN = 256, kStages = 3;
+constexpr int kTileThreads = 512, kTileN = 256;
 constexpr int kTileMaxGroups = 16384;       // offsets within a tile fit 32 bits
 
 // Scale bytes turned into the matrix instruction's order: for every K step and every 64 rows, 64 words
@@ -311,7 +311,7 @@ template <int FA> __device__ __forceinline__ f32x4 scaled_mfma(const i32x8& fb, 
 // in four parts of 16 lanes, {0-3, 12-15, 20-27}, {4-11, 16-19, 28-31} and the same
 // 32 lanes on (measured), from 64 banks; with the row's low three bits (rows of 128
 // bytes) or its bits 1 and 2 (64 bytes) in the chunk number no part meets a bank twice.
-template <int FA, bool EXACT, int WM> struct Tile {
+template <int FA, bool EXACT, int WM, int STAGES> struct Tile {
     static constexpr int M = 64 * WM, WN = 8 / WM, NT = kTileN / WN / 16, MT = 4;
     static constexpr int kRowA = FA == kMxFp4 ? 64 : 128;       // bytes of a row of A a step
     static constexpr int kBytesA = M * kRowA, kBytesB = kTileN * 64;
@@ -324,9 +324,9 @@ template <int FA, bool EXACT, int WM> struct Tile {
     static __device__ __forceinline__ int piece_a(int wave, int i) { return (wave * kLoadsA + i) % (kBytesA / 1024); }
 };
 
-template <int FA, bool EXACT, int WM, typename TO>
-__global__ __launch_bounds__(kTileThreads, 2) void mx_matmul_tile_kernel(TileArgs p) {
-    using S = Tile<FA, EXACT, WM>;
+template <int FA, bool EXACT, int WM, int STAGES, int PER_CU, typename TO>
+__global__ __launch_bounds__(kTileThreads, 2 * PER_CU) void mx_matmul_tile_kernel(TileArgs p) {
+    using S = Tile<FA, EXACT, WM, STAGES>;
     extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
     const int lane = threadIdx.x & 63, r = lane & 15, g = lane >> 4;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -413,12 +413,16 @@ __global__ __launch_bounds__(kTileThreads, 2) void mx_matmul_tile_kernel(TileArg
         const auto read_b = [&](const unsigned char* st, int i) {
             fb[i] = *reinterpret_cast<const i32x4*>(st + S::kBytesA + ((wn * S::NT + i) * 16 + r) * 64 + ((g ^ ((r >> 1) & 3)) << 4));
         };
-        constexpr int H = S::NT / 2, kReadsA = FA == kMxFp4 ? 1 : 2, kPer = (S::kLoads + S::MT - 1) / S::MT;
+        constexpr int H = S::NT / 2, kReadsA = FA == kMxFp4 ? 1 : 2;
+        // Loads of a step that go out in a second half; the rest goes out in the next first half.  Half of them where the
+        // multiplications of half a step are over before all loads are out: 4-bit rows in the tall tile (2048 x 131072 x
+        // 4096 672 -> 650 us; short products, which the tall tile is not for, would lose by the later start).
+        constexpr int kEarly = FA == kMxFp4 && WM == 4 ? (S::kLoads + 1) / 2 : S::kLoads;
 #pragma unroll
-        for (int s = 0; s < 3; ++s)
+        for (int s = 0; s < STAGES; ++s)
 #pragma unroll
-            for (int i = 0; i < S::kLoads; ++i) request(i, step_at(s), smem + s * S::kStage);
-        asm volatile("s_waitcnt vmcnt(%0)" ::"n"(2 * S::kLoads) : "memory");
+            for (int i = 0; i < (s < STAGES - 1 ? S::kLoads : kEarly); ++i) request(i, step_at(s), smem + s * S::kStage);
+        asm volatile("s_waitcnt vmcnt(%0)" ::"n"((STAGES - 2) * S::kLoads + kEarly) : "memory");
         barrier_keeping_loads();
         unsigned int xa, xb[kWords];
         read_words(smem, xa, xb);
@@ -429,11 +433,14 @@ __global__ __launch_bounds__(kTileThreads, 2) void mx_matmul_tile_kernel(TileArg
         int now = 0;
         for (int k = 0; k < p.groups; ++k) {
             unsigned char* st = smem + now * S::kStage;
-            now = now == 2 ? 0 : now + 1;
+            unsigned char* before = smem + (now == 0 ? STAGES - 1 : now - 1) * S::kStage;
+            now = now == STAGES - 1 ? 0 : now + 1;
             const unsigned char* st1 = smem + now * S::kStage;
-            // first half: the second half's operands of B come in
+            // first half: the second half's operands of B come in, the rest of the last step's loads goes out
 #pragma unroll
             for (int i = H; i < S::NT; ++i) read_b(st, i);
+#pragma unroll
+            for (int l = kEarly; l < S::kLoads; ++l) request(l, step_at(k + STAGES - 1), before);
 #pragma unroll
             for (int i = 0; i < H; ++i)
 #pragma unroll
@@ -442,12 +449,18 @@ __global__ __launch_bounds__(kTileThreads, 2) void mx_matmul_tile_kernel(TileArg
                                                 i % 4, xa, j);
 #pragma unroll
             for (int i = 0; i < H; ++i) {
-                __builtin_amdgcn_sched_group_barrier(0x008, S::MT / 2, 0);
+                __builtin_amdgcn_sched_group_barrier(0x008, 2, 0);
                 __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
-                __builtin_amdgcn_sched_group_barrier(0x008, S::MT / 2, 0);
+                __builtin_amdgcn_sched_group_barrier(0x008, kEarly < S::kLoads ? 0 : 2, 0);
+            }
+            constexpr int kLate = S::kLoads - kEarly, kBetween = 2 * H / (kLate + 1) > 0 ? 2 * H / (kLate + 1) : 1;
+#pragma unroll
+            for (int l = 0; l < kLate; ++l) {
+                __builtin_amdgcn_sched_group_barrier(0x008, kBetween, 0);
+                __builtin_amdgcn_sched_group_barrier(0x020, 1, 0);
             }
             // Everybody is done reading step k, and step k + 1 has landed for everybody.
-            asm volatile("s_waitcnt vmcnt(%0)" ::"n"(S::kLoads) : "memory");
+            asm volatile("s_waitcnt vmcnt(%0)" ::"n"((STAGES - 2) * S::kLoads) : "memory");
             barrier_keeping_loads();
             // second half, A's operands outside: each is replaced by the next step's as soon as it is used up, B's first
             // half too, and the loads of step k + 3 go out between (one holds its wave up for 100 to 200 cycles)
@@ -462,20 +475,20 @@ __global__ __launch_bounds__(kTileThreads, 2) void mx_matmul_tile_kernel(TileArg
                 read_a(st1, j);
                 if (j < H) read_b(st1, j);
 #pragma unroll
-                for (int l = j * kPer; l < (j + 1) * kPer && l < S::kLoads; ++l) request(l, step_at(k + 3), st);
+                for (int l = j * kEarly / S::MT; l < (j + 1) * kEarly / S::MT; ++l) request(l, step_at(k + STAGES), st);
             }
             __builtin_amdgcn_sched_group_barrier(0x100, 1 + kWords, 0);
 #pragma unroll
             for (int j = 0; j < H; ++j) {
                 __builtin_amdgcn_sched_group_barrier(0x008, S::NT - H, 0);
                 __builtin_amdgcn_sched_group_barrier(0x100, kReadsA + 1, 0);
-                __builtin_amdgcn_sched_group_barrier(0x020, kPer, 0);
+                __builtin_amdgcn_sched_group_barrier(0x020, (kEarly + S::MT - 1) / S::MT, 0);
             }
 #pragma unroll
             for (int j = H; j < S::MT; ++j) {
                 __builtin_amdgcn_sched_group_barrier(0x008, S::NT - H, 0);
                 __builtin_amdgcn_sched_group_barrier(0x100, kReadsA, 0);
-                __builtin_amdgcn_sched_group_barrier(0x020, kPer, 0);
+                __builtin_amdgcn_sched_group_barrier(0x020, (kEarly + S::MT - 1) / S::MT, 0);
             }
             xa = ya;
 #pragma unroll
@@ -599,18 +612,33 @@ template <int FA, typename TO> hipError_t rows_shaped(const MatmulArgs& p, hipSt
 
 long long up(long long x, long long to) { return (x + to - 1) / to * to; }
 
-template <int FA, bool EXACT, int WM, typename TO> hipError_t launch_tiles(TileArgs p, hipStream_t stream) {
-    using S = Tile<FA, EXACT, WM>;
-    constexpr int lds = kStages * S::kStage;
-    const void* fn = reinterpret_cast<const void*>(&mx_matmul_tile_kernel<FA, EXACT, WM, TO>);
-    static_assert(lds <= 160 * 1024, "LDS");
+template <int FA, bool EXACT, int WM, int STAGES, int PER_CU, typename TO> hipError_t launch_tiles(TileArgs p, hipStream_t stream) {
+    using S = Tile<FA, EXACT, WM, STAGES>;
+    constexpr int lds = STAGES * S::kStage;
+    const void* fn = reinterpret_cast<const void*>(&mx_matmul_tile_kernel<FA, EXACT, WM, STAGES, PER_CU, TO>);
+    static_assert(PER_CU * lds <= 160 * 1024 && 8 * 16 * (S::NT * 16 + 4) * 4 <= lds, "LDS");
     const hipError_t e = hipFuncSetAttribute(fn, hipFuncAttributeMaxDynamicSharedMemorySize, lds);
     if (e != hipSuccess) return e;
     p.m_tiles = (int)((p.m + S::M - 1) / S::M);
     const long long tiles = p.m_tiles * ((p.n + kTileN - 1) / kTileN);
     if (tiles > 0x7fffffff) return hipErrorInvalidValue;
-    hipLaunchKernelGGL((mx_matmul_tile_kernel<FA, EXACT, WM, TO>), dim3((unsigned int)tiles), dim3(kTileThreads), lds, stream, p);
+    hipLaunchKernelGGL((mx_matmul_tile_kernel<FA, EXACT, WM, STAGES, PER_CU, TO>), dim3((unsigned int)tiles), dim3(kTileThreads), lds, stream, p);
     return hipGetLastError();
+}
+
+// Tiles of 64, 128 or 256 rows of A.  4-bit rows have room for two workgroups of the 128-row tile a CU, whose starts and
+// ends overlap, and take it where these weigh: short rows, or fewer tall tiles than CUs (measured, us, two workgroups /
+// tall: 511 x 100003 x 768 62 / 70, 1024 x 8192 x 4096 31 / 37, 2048 x 131072 x 4096 764 / 650).
+template <typename TO> hipError_t tiles_4bit(const TileArgs& p, hipStream_t stream) {
+    if (p.m <= 64) return launch_tiles<kMxFp4, false, 1, 3, 1, TO>(p, stream);
+    const long long tall = (p.m + 255) / 256 * ((p.n + kTileN - 1) / kTileN);
+    if (p.m <= 128 || p.groups <= 8 || tall < 256) return launch_tiles<kMxFp4, false, 2, 3, 2, TO>(p, stream);
+    return launch_tiles<kMxFp4, false, 4, 3, 1, TO>(p, stream);
+}
+template <bool EXACT, typename TO> hipError_t tiles_8bit(const TileArgs& p, hipStream_t stream) {
+    if (p.m <= 64) return launch_tiles<kMxFp8, EXACT, 1, 3, 1, TO>(p, stream);
+    if (p.m <= 128) return launch_tiles<kMxFp8, EXACT, 2, 3, 1, TO>(p, stream);
+    return launch_tiles<kMxFp8, EXACT, 4, 3, 1, TO>(p, stream);
 }
 
 }  // namespace
@@ -635,14 +663,8 @@ hipError_t launch_mx_matmul(const void* a_values, const void* a_scales, int a_fo
         const dim3 turn_grid((unsigned int)((up(m, 256) + up(n, 256)) / 64), (unsigned int)((groups + 31) / 32));
         hipLaunchKernelGGL(turn_scales_kernel, turn_grid, dim3(256), 0, stream, ta, tb, groups);
         const TileArgs p{a, b, as, bs, m, n, up(m, 256), up(n, 256), groups, 0, out, ld_out, whole};
-#define MTR_TILES(F, X, T) return m <= 64 ? launch_tiles<F, X, 1, T>(p, stream) : m <= 128 ? launch_tiles<F, X, 2, T>(p, stream) : launch_tiles<F, X, 4, T>(p, stream)
-        if (a_format == kMxFp4) {
-            if (out_dtype == 0) MTR_TILES(kMxFp4, false, float);
-            MTR_TILES(kMxFp4, false, bf16_t);
-        }
-        if (out_dtype == 0) MTR_TILES(kMxFp8, true, float);
-        MTR_TILES(kMxFp8, false, bf16_t);
-#undef MTR_TILES
+        if (a_format == kMxFp4) return out_dtype == 0 ? tiles_4bit<float>(p, stream) : tiles_4bit<bf16_t>(p, stream);
+        return out_dtype == 0 ? tiles_8bit<true, float>(p, stream) : tiles_8bit<false, bf16_t>(p, stream);
     }
     const MatmulArgs p{a, static_cast<const unsigned char*>(a_scales), b, static_cast<const unsigned char*>(b_scales), m, n, groups, out, ld_out, whole};
     if (out_dtype == 0) return a_format == kMxFp4 ? rows_shaped<kMxFp4, float>(p, stream) : rows_shaped<kMxFp8, float>(p, stream);
