@@ -27,14 +27,9 @@ namespace mtr {
 namespace {
 
 using u64 = unsigned long long;
-constexpr int kThreads = 256, kWaves = kThreads / 64, kJoinThreads = 1024;
+constexpr int kJoinThreads = 1024;
 constexpr float kLog2e = 1.4426950408889634f;
 
-__device__ __forceinline__ u64 key_of(float v, unsigned int id) {
-    const unsigned int b = __float_as_uint(v + 0.f);     // -0 becomes 0: they are equal
-    const unsigned int o = b & 0x80000000u ? ~b : b | 0x80000000u;
-    return ((u64)o << 32) | (0xffffffffu - id);
-}
 __device__ __forceinline__ float value_of(u64 key) {
     const unsigned int o = (unsigned int)(key >> 32);
     return __uint_as_float(o & 0x80000000u ? o & 0x7fffffffu : ~o);
@@ -46,9 +41,22 @@ __device__ __forceinline__ u64 lane_key(u64 key, int lane) {     // lane is wave
     const unsigned int hi = __builtin_amdgcn_readlane((int)(unsigned int)(key >> 32), lane);
     return ((u64)hi << 32) | lo;
 }
-__device__ __forceinline__ u64 shuffle_key(u64 key, int lane) {
-    const unsigned int lo = __shfl((int)(unsigned int)key, lane, 64), hi = __shfl((int)(unsigned int)(key >> 32), lane, 64);
-    return ((u64)hi << 32) | lo;
+// The value of lane (own ^ D), without a trip through LDS.
+template <int D> __device__ __forceinline__ unsigned int across(unsigned int v, int lane) {
+    if constexpr (D == 1) return dpp<0xB1>(v);                      // quad_perm 1 0 3 2
+    if constexpr (D == 2) return dpp<0x4E>(v);                      // quad_perm 2 3 0 1
+    if constexpr (D == 4) return dpp<0x1B>(dpp<0x141>(v));          // ^7 (row_half_mirror), then ^3 (quad_perm 3 2 1 0)
+    if constexpr (D == 8) return dpp<0x128>(v);                     // row_ror 8
+    if constexpr (D == 16) {
+        const auto s = __builtin_amdgcn_permlane16_swap(v, v, false, false);   // {even 16s twice, odd 16s twice}
+        return lane & 16 ? s[0] : s[1];
+    }
+    const auto s = __builtin_amdgcn_permlane32_swap(v, v, false, false);
+    return lane & 32 ? s[0] : s[1];
+}
+template <int D> __device__ __forceinline__ u64 exchanged(u64 c, int lane) {
+    const u64 o = ((u64)across<D>((unsigned int)(c >> 32), lane) << 32) | across<D>((unsigned int)c, lane);
+    return ((lane & D) == 0) == (c > o) ? c : o;                    // the larger one to the lane before
 }
 
 // Of two sorted lists of 64 (one key a lane, best in lane 0; the second one REVERSED,
@@ -56,13 +64,12 @@ __device__ __forceinline__ u64 shuffle_key(u64 key, int lane) {
 // a bitonic sequence, which six exchanges sort.
 __device__ __forceinline__ u64 merge_reversed(u64 a, u64 reversed, int lane) {
     u64 c = a > reversed ? a : reversed;
-#pragma unroll
-    for (int d = 32; d >= 1; d >>= 1) {
-        const u64 o = shuffle_key(c, lane ^ d);
-        const bool first = (lane & d) == 0;
-        c = (first == (c > o)) ? c : o;
-    }
-    return c;
+    c = exchanged<32>(c, lane);
+    c = exchanged<16>(c, lane);
+    c = exchanged<8>(c, lane);
+    c = exchanged<4>(c, lane);
+    c = exchanged<2>(c, lane);
+    return exchanged<1>(c, lane);
 }
 
 // A sorted list of 64 with one more key: everything below it moves one lane on.
@@ -74,16 +81,28 @@ __device__ __forceinline__ u64 inserted(u64 key, u64 cand) {
     return key > c ? key : c;
 }
 
-// A lower bound of the k-th largest of the 64 lanes' values (their upper 16 bits'), as the smallest key
-// of that value less one; 0 if there are not k finite ones.
-__device__ __forceinline__ u64 kth_of_lanes(float v, int k) {
+__device__ __forceinline__ unsigned int ordered(float v) {      // larger bits for larger values, equal ones for zeros of both signs
     const unsigned int b = __float_as_uint(v + 0.f);
-    const unsigned int o = b & 0x80000000u ? ~b : b | 0x80000000u;
+    return b & 0x80000000u ? ~b : b | 0x80000000u;
+}
+
+__device__ __forceinline__ u64 key_of(float v, unsigned int id) { return ((u64)ordered(v) << 32) | (0xffffffffu - id); }
+
+// A value that at least k of 256 (four a lane) reach, close below the k-th largest: its upper 12 bits, the rest zero. -inf
+// if there are not k finite ones.  k logits of different parts of the lanes' reach it, so no smaller one is among the k best.
+__device__ __forceinline__ float floor_of(const float (&v)[4], int k) {
+    const unsigned int o[4] = {ordered(v[0]), ordered(v[1]), ordered(v[2]), ordered(v[3])};
     unsigned int t = 0;
 #pragma unroll
-    for (int bit = 31; bit >= 16; --bit)
-        if (__popcll(__ballot(o >= (t | (1u << bit)))) >= k) t |= 1u << bit;
-    return t > 0x007fffffu ? (u64)t << 32 : 0;      // 0x007fffff is -inf
+    for (int bit = 31; bit >= 20; --bit) {
+        const unsigned int c = t | (1u << bit);
+        int n = 0;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) n += __popcll(__ballot(o[i] >= c));
+        t = n >= k ? c : t;
+    }
+    if (t <= 0x007fffffu) return -INFINITY;
+    return __uint_as_float(t & 0x80000000u ? t & 0x7fffffffu : ~t);
 }
 
 struct Sums {       // of one part of a row
@@ -157,33 +176,17 @@ __device__ __forceinline__ void write_row(const Outputs& o, long long row, const
     }
 }
 
-// 16 bytes of logits from element e on; outside [e0, e1) excluded ones.
 template <typename T> struct alignas(16) Piece { T v[16 / sizeof(T)]; };
-template <typename T> __device__ __forceinline__ T excluded();
-template <> __device__ __forceinline__ float excluded<float>() { return -INFINITY; }
-template <> __device__ __forceinline__ bf16_t excluded<bf16_t>() { return 0xff80; }
-template <> __device__ __forceinline__ _Float16 excluded<_Float16>() { return (_Float16)-INFINITY; }
-template <typename T> __device__ __forceinline__ Piece<T> load_piece(const T* l, long long e, long long e0, long long e1) {
-    constexpr int N = 16 / sizeof(T);
-    Piece<T> p;
-    if (e >= e0 && e + N <= e1) {
-        p = *reinterpret_cast<const Piece<T>*>(l + e);
-    } else {
-#pragma unroll
-        for (int i = 0; i < N; ++i) p.v[i] = e + i >= e0 && e + i < e1 ? l[e + i] : excluded<T>();
-    }
-    return p;
-}
 
 // One workgroup a part of a row.  part_sums / part_keys: [row][split] and
 // [row][split][top_k]; with one split the row is finished here instead.
-template <typename T, bool TOP>
-__global__ __launch_bounds__(kThreads) void token_logprobs_kernel(Outputs o, int splits, long long part_len,
+template <typename T, bool TOP, int WAVES>
+__global__ __launch_bounds__(64 * WAVES) void token_logprobs_kernel(Outputs o, int splits, long long part_len,
                                                                   Sums* __restrict__ part_sums, u64* __restrict__ part_keys) {
     constexpr int EPC = 16 / sizeof(T);                 // elements of a 16-byte load
-    constexpr int U = sizeof(T) == 2 ? 2 : 4;           // loads a lane and round: 16 logits
-    __shared__ Sums wave_sums[kWaves];
-    __shared__ u64 wave_keys[TOP ? kWaves * 64 : 1];
+    constexpr int U = 4;                                // loads a lane and round
+    __shared__ Sums wave_sums[WAVES];
+    __shared__ u64 wave_keys[TOP ? WAVES * 64 : 1];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     const long long row = blockIdx.x / splits;
     const int split = (int)(blockIdx.x - row * splits);
@@ -199,46 +202,61 @@ __global__ __launch_bounds__(kThreads) void token_logprobs_kernel(Outputs o, int
     float ref = 0.f;                                    // m, or 0 while there is none
     u64 key = 0, kth = 0;                               // this lane's place of the list, and the k-th best
 
-    long long c0 = (long long)wave * 64 * U;
-    Piece<T> next[U];
-#pragma unroll
-    for (int u = 0; u < U; ++u) next[u] = load_piece<T>(l, base + (c0 + u * 64 + lane) * EPC, e0, e1);
-    for (; c0 < chunks; c0 += (long long)kThreads * U) {
+    for (long long c0 = (long long)wave * 64 * U; c0 < chunks; c0 += 64ll * WAVES * U) {
         float x[U * EPC];
+        const long long first = base + c0 * EPC;        // the round's first element; lane by lane 16 bytes, U times
+        if (first >= e0 && first + 64 * U * EPC <= e1) {        // wave-uniform: all of it is there
+            const Piece<T>* p = reinterpret_cast<const Piece<T>*>(l + first) + lane;
 #pragma unroll
-        for (int u = 0; u < U; ++u)
+            for (int u = 0; u < U; ++u) {
+                const Piece<T> v = __builtin_bit_cast(Piece<T>, __builtin_nontemporal_load(reinterpret_cast<const u32x4*>(p + u * 64)));
 #pragma unroll
-            for (int i = 0; i < EPC; ++i) x[u * EPC + i] = to_f32<T>(next[u].v[i]);
-        if (c0 + (long long)kThreads * U < chunks) {    // the next round's loads before this one's arithmetic
+                for (int i = 0; i < EPC; ++i) x[u * EPC + i] = to_f32<T>(v.v[i]);
+            }
+        } else {
 #pragma unroll
-            for (int u = 0; u < U; ++u) next[u] = load_piece<T>(l, base + (c0 + (long long)kThreads * U + u * 64 + lane) * EPC, e0, e1);
+            for (int u = 0; u < U; ++u) {
+                const long long e = first + (u * 64 + lane) * EPC;
+                if (e >= e0 && e + EPC <= e1) {
+                    const Piece<T> v = *reinterpret_cast<const Piece<T>*>(l + e);
+#pragma unroll
+                    for (int i = 0; i < EPC; ++i) x[u * EPC + i] = to_f32<T>(v.v[i]);
+                } else {
+#pragma unroll
+                    for (int i = 0; i < EPC; ++i) x[u * EPC + i] = e + i >= e0 && e + i < e1 ? to_f32<T>(l[e + i]) : -INFINITY;
+                }
+            }
         }
-        float top = x[0];
+        float tops[4];                                  // of quarters of the lane's logits
 #pragma unroll
-        for (int i = 1; i < U * EPC; ++i) top = fmaxf(top, x[i]);
+        for (int q = 0; q < 4; ++q) {
+            tops[q] = x[q * (U * EPC / 4)];
+#pragma unroll
+            for (int i = 1; i < U * EPC / 4; ++i) tops[q] = fmaxf(tops[q], x[q * (U * EPC / 4) + i]);
+        }
+        const float top = fmaxf(fmaxf(tops[0], tops[1]), fmaxf(tops[2], tops[3]));
         if (__ballot(top > above)) {                    // wave-uniform, rare
             float m = sums.m;
             if constexpr (TOP) {
-                if (kth == 0) kth = kth_of_lanes(top, o.top_k);
+                float least = above;                    // candidates reach it
+                if (kth == 0) least = floor_of(tops, o.top_k);
 #pragma unroll
                 for (int i = 0; i < U * EPC; ++i) {
-                    const unsigned int id = (unsigned int)(base + (c0 + (i / EPC) * 64 + lane) * EPC + i % EPC);
-                    const u64 mine = x[i] > -INFINITY ? key_of(x[i], id) : 0;
-                    u64 mask = __ballot(mine > kth);
+                    u64 mask = __ballot(x[i] >= least && x[i] > -INFINITY);
                     while (mask) {
-                        const u64 cand = lane_key(mine, __ffsll((long long)mask) - 1);
+                        const int from = __ffsll((long long)mask) - 1;
                         mask &= mask - 1;
+                        const float v = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(x[i]), from));
+                        const u64 cand = key_of(v, (unsigned int)(first + (i / EPC * 64 + from) * EPC + i % EPC));
                         if (cand > kth) {
                             key = inserted(key, cand);
-                            const u64 last = lane_key(key, o.top_k - 1);
-                            kth = last > kth ? last : kth;
+                            kth = lane_key(key, o.top_k - 1);
                         }
                     }
                 }
-                const u64 best = lane_key(key, 0), last = lane_key(key, o.top_k - 1);
+                const u64 best = lane_key(key, 0);
                 m = best ? value_of(best) : -INFINITY;
-                above = last ? value_of(last) : -INFINITY;
-                kth = last;
+                above = kth ? value_of(kth) : -INFINITY;
             } else {
                 m = fmaxf(m, top);
 #pragma unroll
@@ -264,7 +282,7 @@ __global__ __launch_bounds__(kThreads) void token_logprobs_kernel(Outputs o, int
         sums.s += __shfl_xor(sums.s, off, 64);
         sums.t += __shfl_xor(sums.t, off, 64);
     }
-    join_waves<kWaves, TOP>(sums, key, wave_sums, wave_keys, wave, lane);
+    join_waves<WAVES, TOP>(sums, key, wave_sums, wave_keys, wave, lane);
     if (wave != 0) return;
     if (splits == 1) {
         write_row<T>(o, row, sums, key, lane);
@@ -300,34 +318,46 @@ __global__ __launch_bounds__(kJoinThreads) void token_logprobs_join_kernel(Outpu
     if (wave == 0) write_row<T>(o, row, sums, key, lane);
 }
 
-// Parts a row: about four workgroups per CU in all, parts of at least 4096 logits.
-int splits_for(long long n, long long v) {
-    long long want = (1024 + n - 1) / n;
-    const long long most = v / 4096 > 1 ? v / 4096 : 1;
-    return (int)(want < most ? want : most);
+// How rows are cut (measured, microseconds).  Waves of a workgroup, one a row: 4 for short rows (4096 x 8000 bf16 28, with
+// 8 44, with 16 76) and where there are rows for every CU several times over (2048 x 100003 bf16 84 / 91 / 101), 8 there
+// from about 200 KB a row on (2048 x 131072 bf16 116 / 104 / 114), 16 for fewer long rows (256 x 131072 fp32 41 / 28 / 26).
+// Parts of a row, of four waves and at least 4096 logits, only for less than 128 rows that are longer still, as a second
+// launch then joins them (1 x 131072 fp32, 20 alternatives: 15 in 32 parts, 36 whole; 63 x 50257 fp16: 16 in 12 parts, 15 whole).
+struct Cut {
+    int waves, splits;
+};
+Cut cut_for(long long n, long long v, int size) {
+    if (v <= 8192) return {4, 1};
+    if (n >= 1024) return {v * size >= 200000 ? 8 : 4, 1};
+    if (n >= 128) return {v > 32768 ? 16 : 8, 1};
+    if (v <= 65536) return {16, 1};
+    const long long want = (1024 + n - 1) / n, most = v / 4096;
+    return {4, (int)(want < most ? want : most)};
 }
 
-template <typename T> hipError_t launch_typed(const Outputs& o, long long n, void* workspace, hipStream_t stream) {
-    const int splits = splits_for(n, o.v);
-    const long long part_len = (o.v + splits - 1) / splits;
+template <typename T, bool TOP> hipError_t launch_shaped(const Outputs& o, long long n, void* workspace, hipStream_t stream) {
+    const Cut c = cut_for(n, o.v, sizeof(T));
+    const long long part_len = (o.v + c.splits - 1) / c.splits;
     Sums* sums = static_cast<Sums*>(workspace);
     u64* keys = nullptr;
-    if (splits > 1) keys = reinterpret_cast<u64*>(static_cast<char*>(workspace) + (n * splits * (long long)sizeof(Sums) + 7) / 8 * 8);
-    const dim3 grid((unsigned int)(n * splits));
-    if (o.top_k) hipLaunchKernelGGL((token_logprobs_kernel<T, true>), grid, dim3(kThreads), 0, stream, o, splits, part_len, sums, keys);
-    else hipLaunchKernelGGL((token_logprobs_kernel<T, false>), grid, dim3(kThreads), 0, stream, o, splits, part_len, sums, keys);
-    if (splits > 1) {
-        if (o.top_k) hipLaunchKernelGGL((token_logprobs_join_kernel<T, true>), dim3((unsigned int)n), dim3(kJoinThreads), 0, stream, o, splits, sums, keys);
-        else hipLaunchKernelGGL((token_logprobs_join_kernel<T, false>), dim3((unsigned int)n), dim3(kJoinThreads), 0, stream, o, splits, sums, keys);
-    }
+    if (c.splits > 1) keys = reinterpret_cast<u64*>(static_cast<char*>(workspace) + (n * c.splits * (long long)sizeof(Sums) + 7) / 8 * 8);
+    const dim3 grid((unsigned int)(n * c.splits));
+    if (c.waves == 16) hipLaunchKernelGGL((token_logprobs_kernel<T, TOP, 16>), grid, dim3(1024), 0, stream, o, c.splits, part_len, sums, keys);
+    else if (c.waves == 8) hipLaunchKernelGGL((token_logprobs_kernel<T, TOP, 8>), grid, dim3(512), 0, stream, o, c.splits, part_len, sums, keys);
+    else hipLaunchKernelGGL((token_logprobs_kernel<T, TOP, 4>), grid, dim3(256), 0, stream, o, c.splits, part_len, sums, keys);
+    if (c.splits > 1)
+        hipLaunchKernelGGL((token_logprobs_join_kernel<T, TOP>), dim3((unsigned int)n), dim3(kJoinThreads), 0, stream, o, c.splits, sums, keys);
     return hipGetLastError();
+}
+template <typename T> hipError_t launch_typed(const Outputs& o, long long n, void* workspace, hipStream_t stream) {
+    return o.top_k ? launch_shaped<T, true>(o, n, workspace, stream) : launch_shaped<T, false>(o, n, workspace, stream);
 }
 
 }  // namespace
 
 long long token_logprobs_workspace(long long n, long long v, int top_k) {
     if (n < 1 || v < 1) return 0;
-    const int splits = splits_for(n, v);
+    const int splits = cut_for(n, v, 2).splits;     // of every type alike
     if (splits == 1) return 0;
     return (n * splits * (long long)sizeof(Sums) + 7) / 8 * 8 + n * splits * top_k * 8;
 }
