@@ -88,17 +88,19 @@ __device__ __forceinline__ unsigned int ordered(float v) {      // larger bits f
 
 __device__ __forceinline__ u64 key_of(float v, unsigned int id) { return ((u64)ordered(v) << 32) | (0xffffffffu - id); }
 
-// A value that at least k of 256 (four a lane) reach, close below the k-th largest: its upper 12 bits, the rest zero. -inf
+// A value that at least k of 64 N (N a lane) reach, close below the k-th largest: its upper 12 bits, the rest zero. -inf
 // if there are not k finite ones.  k logits of different parts of the lanes' reach it, so no smaller one is among the k best.
-__device__ __forceinline__ float floor_of(const float (&v)[4], int k) {
-    const unsigned int o[4] = {ordered(v[0]), ordered(v[1]), ordered(v[2]), ordered(v[3])};
+template <int N> __device__ __forceinline__ float floor_of(const float (&v)[N], int k) {
+    unsigned int o[N];
+#pragma unroll
+    for (int i = 0; i < N; ++i) o[i] = ordered(v[i]);
     unsigned int t = 0;
 #pragma unroll
     for (int bit = 31; bit >= 20; --bit) {
         const unsigned int c = t | (1u << bit);
         int n = 0;
 #pragma unroll
-        for (int i = 0; i < 4; ++i) n += __popcll(__ballot(o[i] >= c));
+        for (int i = 0; i < N; ++i) n += __popcll(__ballot(o[i] >= c));
         t = n >= k ? c : t;
     }
     if (t <= 0x007fffffu) return -INFINITY;
@@ -239,18 +241,26 @@ __global__ __launch_bounds__(64 * WAVES) void token_logprobs_kernel(Outputs o, i
             float m = sums.m;
             if constexpr (TOP) {
                 float least = above;                    // candidates reach it
-                if (kth == 0) least = floor_of(tops, o.top_k);
+                if (kth == 0) {                         // a few of 64 parts' maxima say little less than of 256 parts'
+                    const float one[1] = {top};
+                    least = o.top_k <= 16 ? floor_of(one, o.top_k) : floor_of(tops, o.top_k);
+                }
+                least = fmaxf(least, -3.402823466e38f); // -inf is no candidate
 #pragma unroll
-                for (int i = 0; i < U * EPC; ++i) {
-                    u64 mask = __ballot(x[i] >= least && x[i] > -INFINITY);
-                    while (mask) {
-                        const int from = __ffsll((long long)mask) - 1;
-                        mask &= mask - 1;
-                        const float v = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(x[i]), from));
-                        const u64 cand = key_of(v, (unsigned int)(first + (i / EPC * 64 + from) * EPC + i % EPC));
-                        if (cand > kth) {
-                            key = inserted(key, cand);
-                            kth = lane_key(key, o.top_k - 1);
+                for (int q = 0; q < 4; ++q) {
+                    if (!__ballot(tops[q] >= least)) continue;
+#pragma unroll
+                    for (int i = q * (U * EPC / 4); i < (q + 1) * (U * EPC / 4); ++i) {
+                        u64 mask = __ballot(x[i] >= least);
+                        while (mask) {
+                            const int from = __ffsll((long long)mask) - 1;
+                            mask &= mask - 1;
+                            const float v = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(x[i]), from));
+                            const u64 cand = key_of(v, (unsigned int)(first + (i / EPC * 64 + from) * EPC + i % EPC));
+                            if (cand > kth) {
+                                key = inserted(key, cand);
+                                kth = lane_key(key, o.top_k - 1);
+                            }
                         }
                     }
                 }
