@@ -34,14 +34,22 @@ def top_pages_for_keywords(kw_embeddings_map: dict, pages, top_k: int | None = N
     return {kw: (idx[i], score[i]) for i, (kw, _) in enumerate(usable)}
 
 
-def top_pages_for_texts(keywords: list, model_name: str, device: str, pages, top_k: int = 1, batch_size: int = 64) -> dict:
+def top_pages_for_texts(keywords: list, model_name: str, device: str, pages, top_k: int = 1, batch_size: int = 64,
+                        rerank_model: str | None = None, candidates: int = 20) -> dict:
     """Encoder and retriever on the same GPU: embeds the keyword texts
     (pipeline/async_main.py:195), scores them while still in HBM and brings
     back only the hits.  keyword -> (idx (top_k,), score (top_k,)); {} when
-    there is nothing to embed, the model cannot load or there are no pages."""
+    there is nothing to embed, the model cannot load or there are no pages.
+    rerank_model: a causal language model that re-orders the best `candidates` (at
+    least top_k) pages by how likely it finds the keyword after each (rerank.py)
+    before the best top_k are kept; the scores are then its own."""
     from .local_rag import embed_queries_device
     if not keywords or len(pages) == 0:
         return {}
+    if rerank_model is not None:
+        from .rerank import rerank_hits
+        hits = top_pages_for_texts(keywords, model_name, device, pages, max(top_k, candidates), batch_size)
+        return rerank_hits(hits, pages, rerank_model, device, top_k)
     vectors = embed_queries_device(list(keywords), model_name, device, batch_size)
     if vectors is None:
         return {}

@@ -1,0 +1,60 @@
+"""Re-ranking: what needs no GPU (token arrangement, conventions, refusals)."""
+import logging
+
+import numpy as np
+import pytest
+import torch
+
+
+def test_sequences_cut_the_page_and_never_the_query():
+    from medical_rag_amd.rerank import _sequences
+    rows, begins = _sequences([[1, 2, 3], [], [4] * 50], [7, 8], [9], [0], 10)
+    assert rows == [[0, 1, 2, 3, 9, 7, 8], [0, 9, 7, 8], [0] + [4] * 6 + [9, 7, 8]]
+    assert begins == [5, 2, 8] and all(len(r) <= 10 and r[b:] == [7, 8] for r, b in zip(rows, begins))
+    with pytest.raises(ValueError):
+        _sequences([[1]], [7] * 10, [9], [0], 10)
+
+
+def test_no_hits_and_no_model():
+    from medical_rag_amd import rerank
+    pages = [{"index": i, "text": f"page {i}"} for i in range(4)]
+    for hits in ([], np.array([-1, -1]), [9]):
+        idx, scores = rerank.rerank_pages("q", hits, pages, "unused")
+        assert idx.shape == (0,) and scores.shape == (0,)
+    with pytest.raises(ValueError):
+        rerank.rerank_pages("q", [1, 2], pages, "unused", device="cpu")
+    logging.disable(logging.CRITICAL)
+    try:
+        idx, scores = rerank.rerank_pages("q", [2, -1, 0], pages, "/nonexistent/model/dir")
+    finally:
+        logging.disable(logging.NOTSET)
+    assert idx.tolist() == [2, 0] and np.isnan(scores).all()
+    assert rerank.rerank_hits({}, pages, "unused") == {}
+
+
+def tiny_llama(**extra):
+    from transformers import LlamaConfig, LlamaForCausalLM
+    return LlamaForCausalLM(LlamaConfig(vocab_size=64, hidden_size=32, intermediate_size=48, num_hidden_layers=1, num_attention_heads=2,
+                                        num_key_value_heads=2, max_position_embeddings=64, **extra)).eval()
+
+
+def test_heads_that_compute_something_else_are_refused():
+    from medical_rag_amd.rerank import ScoringHead
+
+    class Centred(torch.nn.Module):
+        def __init__(self, weight):
+            super().__init__()
+            self.weight, self.eps = weight, 1e-6
+
+        def forward(self, x):
+            return torch.nn.functional.layer_norm(x, x.shape[-1:], self.weight)
+
+    for change in (lambda m: setattr(m.model, "norm", Centred(m.model.norm.weight)), lambda m: setattr(m.config, "final_logit_softcapping", 30.0),
+                   lambda m: setattr(m.config, "logit_scale", 0.5), lambda m: setattr(m.model, "norm", torch.nn.Identity()),
+                   lambda m: setattr(m, "lm_head", torch.nn.Linear(32, 64, bias=True)), lambda m: delattr(m.model, "norm")):
+        model = tiny_llama()
+        change(model)
+        with pytest.raises(ValueError):
+            ScoringHead.from_model(model)
+    with pytest.raises(ValueError):     # a plain head, but not on a GPU
+        ScoringHead.from_model(tiny_llama())

@@ -118,10 +118,10 @@ def test_c_refusals_come_before_any_hip_call():
     refuses(mm(o=None), "NULL")
     refuses(mm(ld=1), "stride")
     refuses(mm(m=-1), "shape")
-    assert lib.mtr_mx_matmul_workspace(300, 500, 1000) > 0 and lib.mtr_mx_matmul_workspace(0, 5, 5) == 0
-    refuses(mm(m=300, n=500, d=1000, ld=500), "workspace")
-    refuses(mm(m=300, n=500, d=1000, ld=500, w=at, wb=64), "workspace")
-    refuses(mm(m=300, n=500, d=1000, ld=500, w=at + 2, wb=1 << 30), "workspace")
+    assert lib.mtr_mx_matmul_workspace(3000, 5000, 1000) > 0 and lib.mtr_mx_matmul_workspace(0, 5, 5) == 0
+    refuses(mm(m=3000, n=5000, d=1000, ld=5000), "workspace")
+    refuses(mm(m=3000, n=5000, d=1000, ld=5000, w=at, wb=64), "workspace")
+    refuses(mm(m=3000, n=5000, d=1000, ld=5000, w=at + 2, wb=1 << 30), "workspace")
     assert mm(m=0, o=None) == _native.MTR_OK and mm(n=0, o=None) == _native.MTR_OK
 
     def lp(x=at, dt=0, n=2, v=100, ld=100, t=at, g=1, k=0, l=at, e=at, ti=at, tl=at, w=at, wb=1 << 20):
