@@ -232,16 +232,26 @@ MATMULS = [(1, 1, 1), (1, 16, 32), (1, 1000, 4096), (2, 17, 100), (3, 129, 128),
            (64, 1, 512), (65, 511, 129), (100, 640, 768), (128, 128, 128), (255, 257, 513), (256, 256, 1024), (257, 520, 640), (700, 300, 200)]
 
 
+# results large enough for tiles (more than three million): every tile shape, one K step to many, partial tiles
+TILES = [(64, 50001, 100), (50, 70000, 200), (65, 47003, 384), (128, 24001, 1500), (129, 24000, 256), (513, 6001, 513), (300, 10111, 1030),
+         (700, 24100, 1100), (2100, 1500, 130)]
+
+
+def product(va, vb):
+    """The float64 products, a (m, n) tensor on the GPU."""
+    import torch
+    return torch.from_numpy(va).cuda() @ torch.from_numpy(vb).cuda().t()
+
+
 @pytest.mark.parametrize("out", ["float32", "bfloat16"])
 @pytest.mark.parametrize("fmt", ["mxfp8", "mxfp4"])
 def test_matmul_of_whole_numbers_is_exact(sc, fmt, out):
     import torch
-    for i, (m, n, d) in enumerate(MATMULS):
+    for i, (m, n, d) in enumerate(MATMULS + TILES):
         a, va = stored(sc, m, d, fmt, seed=i, exact=True)
         b, vb = stored(sc, n, d, "mxfp4", seed=100 + i, exact=True)
         got = sc.mx_matmul(a, b, getattr(torch, out))
-        want = torch.from_numpy(va @ vb.T).to(getattr(torch, out))
-        assert torch.equal(got.cpu(), want), (m, n, d)
+        assert torch.equal(got, product(va, vb).to(getattr(torch, out))), (m, n, d)
 
 
 def check_matmul(got, va, vb, fmt):
@@ -250,14 +260,16 @@ def check_matmul(got, va, vb, fmt):
     come from the matrix instruction that keeps 2^-16 of its largest product: 128
     of them per step then add 2^-9 of the largest |a b| at most; and every result
     is rounded once."""
-    want, size = va @ vb.T, np.abs(va) @ np.abs(vb).T
+    import torch
+    want, size = product(va, vb), product(np.abs(va), np.abs(vb))
     err = va.shape[1] * U * size
     name = str(got.dtype).replace("torch.", "")
     if name == "bfloat16" and fmt == "mxfp8":
         err = err + 2.0 ** -13 * size
-    assert (np.abs(f64(got) - want) <= err + HALF_STEP[name] * np.abs(want) * (1 + 2.0 ** -7)).all()
+    off = got.double() - want
+    assert bool((off.abs() <= err + HALF_STEP[name] * want.abs() * (1 + 2.0 ** -7)).all())
     # and far better than that over all: roundings do not add up in one direction
-    rel = np.linalg.norm(f64(got) - want) / max(np.linalg.norm(want), 1e-30)
+    rel = float(torch.linalg.norm(off) / torch.linalg.norm(want).clamp(min=1e-30))
     assert rel <= (2e-6 if name == "float32" else 2.0 ** -8), rel
 
 
@@ -265,7 +277,7 @@ def check_matmul(got, va, vb, fmt):
 @pytest.mark.parametrize("fmt", ["mxfp8", "mxfp4"])
 def test_matmul(sc, fmt, out):
     import torch
-    for i, (m, n, d) in enumerate(MATMULS + [(9, 100, 8192), (300, 700, 4096)]):
+    for i, (m, n, d) in enumerate(MATMULS + [(9, 100, 8192), (300, 700, 4096)] + TILES):
         a, va = stored(sc, m, d, fmt, seed=200 + i)
         b, vb = stored(sc, n, d, "mxfp4", seed=300 + i)
         check_matmul(sc.mx_matmul(a, b, getattr(torch, out)), va, vb, fmt)
@@ -274,34 +286,40 @@ def test_matmul(sc, fmt, out):
 @pytest.mark.parametrize("fmt", ["mxfp8", "mxfp4"])
 def test_matmul_into_strided_rows_and_nothing_else(sc, fmt):
     import torch
-    for m, n, d in ((5, 70, 200), (300, 333, 256), (40, 260, 300)):
+    for m, n, d in ((5, 70, 200), (300, 333, 256), (40, 260, 300), (60, 50003, 128), (100, 31001, 200), (300, 10501, 130)):
         a, va = stored(sc, m, d, fmt, seed=1, exact=True)
         b, vb = stored(sc, n, d, "mxfp4", seed=2, exact=True)
         for dtype in (torch.float32, torch.bfloat16):
+            want = product(va, vb).to(dtype)
             for off in (0, 1, 3, 8):
-                whole = torch.full((m + 2, n + 37), -5.0, dtype=dtype, device="cuda")
-                out = whole[1:m + 1, off:off + n]
-                assert sc.mx_matmul(a, b, out=out) is out
-                assert torch.equal(out.cpu(), torch.from_numpy(va @ vb.T).to(dtype))
-                out.fill_(-5.0)
-                assert (whole == -5).all()
+                for more in (37, 44):
+                    whole = torch.full((m + 2, n + more), -5.0, dtype=dtype, device="cuda")
+                    out = whole[1:m + 1, off:off + n]
+                    assert sc.mx_matmul(a, b, out=out) is out
+                    assert torch.equal(out, want)
+                    out.fill_(-5.0)
+                    assert (whole == -5).all()
     a, va = stored(sc, 2, 64, fmt, seed=3, exact=True)
     b, vb = stored(sc, 50, 64, "mxfp4", seed=4, exact=True)
     far = torch.empty(2 ** 31 + 200, dtype=torch.float32, device="cuda").as_strided((2, 50), (2 ** 31 + 40, 1))
-    assert torch.equal(sc.mx_matmul(a, b, out=far).cpu(), torch.from_numpy(va @ vb.T).float())
+    assert torch.equal(sc.mx_matmul(a, b, out=far), product(va, vb).float())
+    a, va = stored(sc, 70, 64, fmt, seed=3, exact=True)
+    b, vb = stored(sc, 50000, 64, "mxfp4", seed=4, exact=True)
+    far = torch.empty(69 * (2 ** 26) + 50000, dtype=torch.bfloat16, device="cuda").as_strided((70, 50000), (2 ** 26, 1))
+    assert torch.equal(sc.mx_matmul(a, b, out=far), product(va, vb).bfloat16())
 
 
 @pytest.mark.parametrize("fmt", ["mxfp8", "mxfp4"])
 def test_matmul_nan_blocks_stay_in_their_rows_and_columns(sc, fmt):
     import torch
-    for m, n, d in ((3, 40, 256), (290, 300, 256)):
+    for m, n, d in ((3, 40, 256), (290, 300, 256), (50, 61000, 256), (290, 11000, 256)):
         a, va = stored(sc, m, d, fmt, seed=5)
         b, vb = stored(sc, n, d, "mxfp4", seed=6)
         a.scales[1, 2] = 255
         b.scales[7, 0] = 255
         for dtype in (torch.float32, torch.bfloat16):
-            got = torch.isnan(sc.mx_matmul(a, b, dtype)).cpu()
-            want = torch.zeros(m, n, dtype=torch.bool)
+            got = torch.isnan(sc.mx_matmul(a, b, dtype))
+            want = torch.zeros(m, n, dtype=torch.bool, device="cuda")
             want[1], want[:, 7] = True, True
             assert torch.equal(got, want)
 
@@ -309,16 +327,25 @@ def test_matmul_nan_blocks_stay_in_their_rows_and_columns(sc, fmt):
 def test_matmul_far_scales(sc):
     """Blocks whose scales are at the ends of their range."""
     import torch
-    for m in (2, 280):
+    for m, n in ((2, 270), (280, 270), (280, 11000)):
         for fmt in ("mxfp8", "mxfp4"):
             a, va = stored(sc, m, 128, fmt, seed=7, exact=True)
-            b, vb = stored(sc, 270, 128, "mxfp4", seed=8, exact=True)
+            b, vb = stored(sc, n, 128, "mxfp4", seed=8, exact=True)
+            want = product(va, vb)
             a.scales.fill_(127 + 100)
             b.scales.fill_(127 - 110)
-            assert torch.equal(sc.mx_matmul(a, b).cpu(), torch.from_numpy(np.ldexp(va @ vb.T, -10)).float())
+            assert torch.equal(sc.mx_matmul(a, b), (want * 2.0 ** -10).float())
             a.scales.fill_(20)
             b.scales.fill_(250)
-            assert torch.equal(sc.mx_matmul(a, b).cpu(), torch.from_numpy(np.ldexp(va @ vb.T, 16)).float())
+            assert torch.equal(sc.mx_matmul(a, b), (want * 2.0 ** 16).float())
+
+
+def test_matmul_result_rows_start_on_128_bytes(sc):
+    import torch
+    a, _ = stored(sc, 3, 64, "mxfp8", seed=1)
+    for n, dtype, stride in ((1023, torch.float32, 1023), (1024, torch.float32, 1024), (1025, torch.float32, 1056), (1025, torch.bfloat16, 1088)):
+        got = sc.mx_matmul(a, stored(sc, n, 64, "mxfp4", seed=2)[0], dtype)
+        assert got.shape == (3, n) and got.stride() == (stride, 1)
 
 
 def test_matmul_rows_of_a_view_and_empty_operands(sc):
