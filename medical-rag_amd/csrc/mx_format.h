@@ -126,25 +126,17 @@ __device__ __forceinline__ unsigned int mx_quantize8(const float (&f)[8], unsign
     return code;
 }
 
-// Eight consecutive elements of a row (element 8 * chunk of the row on) and the
-// four scale bytes of their 128.
-template <int FMT>
-__device__ __forceinline__ void mx_dequantize8(const unsigned int (&q)[FMT == kMxFp4 ? 1 : 2], unsigned int scale_word,
-                                               float (&f)[8]) {
-    const float s = mx_scale((scale_word >> (8 * ((threadIdx.x >> 2) & 3))) & 255u);
+// Four elements (e2m1: 16 bits, e4m3: 32) times their scale.
+template <int FMT> __device__ __forceinline__ void mx_decode4(unsigned int q, float scale, float* f) {
     if constexpr (FMT == kMxFp4) {
-        const auto p0 = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(q[0], 1.f, 0), p1 = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(q[0], 1.f, 1);
-        const auto p2 = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(q[0], 1.f, 2), p3 = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(q[0], 1.f, 3);
-        f[0] = p0[0]; f[1] = p0[1]; f[2] = p1[0]; f[3] = p1[1]; f[4] = p2[0]; f[5] = p2[1]; f[6] = p3[0]; f[7] = p3[1];
+        const auto a = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(q, 1.f, 0), b = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(q, 1.f, 1);
+        f[0] = a[0]; f[1] = a[1]; f[2] = b[0]; f[3] = b[1];
     } else {
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {
-            const auto lo = __builtin_amdgcn_cvt_pk_f32_fp8((int)q[h], false), hi = __builtin_amdgcn_cvt_pk_f32_fp8((int)q[h], true);
-            f[4 * h] = lo[0]; f[4 * h + 1] = lo[1]; f[4 * h + 2] = hi[0]; f[4 * h + 3] = hi[1];
-        }
+        const auto a = __builtin_amdgcn_cvt_pk_f32_fp8((int)q, false), b = __builtin_amdgcn_cvt_pk_f32_fp8((int)q, true);
+        f[0] = a[0]; f[1] = a[1]; f[2] = b[0]; f[3] = b[1];
     }
 #pragma unroll
-    for (int i = 0; i < 8; ++i) f[i] *= s;
+    for (int i = 0; i < 4; ++i) f[i] *= scale;
 }
 
 // ---- launchers ------------------------------------------------------------------

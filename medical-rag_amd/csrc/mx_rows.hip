@@ -21,55 +21,98 @@ template <int FMT> __device__ __forceinline__ void store_group(unsigned char* va
     if (lane16 == 0) reinterpret_cast<unsigned int*>(scales)[group] = word;
 }
 
-// Groups of 128 elements, 16 lanes each.  VEC: rows start on 16 bytes and d is a
-// multiple of 8, so that every chunk of eight is whole or absent.
-template <typename T, int FMT, bool VEC>
+// Groups of 128 elements, 16 lanes each and U in turn, whose loads go out together.  VEC: rows start on 16 bytes and d
+// is a multiple of 8, so that every chunk of eight is whole or absent.
+template <typename T, int FMT, bool VEC, int U>
 __global__ __launch_bounds__(kThreads) void mx_quantize_kernel(const T* __restrict__ x, unsigned int n_groups, unsigned int row_groups,
                                                                int d, long long ld, unsigned char* __restrict__ values,
                                                                unsigned char* __restrict__ scales) {
-    const unsigned int group = blockIdx.x * (kThreads / 16) + threadIdx.x / 16;
-    if (group >= n_groups) return;      // 16 lanes leave together
+    const unsigned int first = blockIdx.x * (kThreads / 16 * U) + threadIdx.x / 16;
     const int lane16 = threadIdx.x & 15;
-    const unsigned int row = group / row_groups;
-    const int col = (int)(group - row * row_groups) * 128 + lane16 * 8;
-    const T* p = x + (long long)row * ld + col;
-    float f[8];
-    if (VEC) {
-        if (col < d) load8<T>(p, f);
-        else
+    float f[U][8];
 #pragma unroll
-            for (int i = 0; i < 8; ++i) f[i] = 0.f;
-    } else {
-        load_some<T>(p, d - col, f);
+    for (int u = 0; u < U; ++u) {
+        const unsigned int group = first + u * (kThreads / 16), row = group / row_groups;
+        const int col = (int)(group - row * row_groups) * 128 + lane16 * 8;
+        const T* p = x + (long long)row * ld + col;
+        if (group >= n_groups) {
+        } else if (!VEC) {
+            load_some<T>(p, d - col, f[u]);
+        } else if (col < d) {
+            load8<T>(p, f[u]);
+        } else {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) f[u][i] = 0.f;
+        }
     }
-    unsigned int q[FMT == kMxFp4 ? 1 : 2];
-    const unsigned int word = mx_quantize8<FMT>(f, q);
-    store_group<FMT>(values, scales, group, lane16, q, word);
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+        const unsigned int group = first + u * (kThreads / 16);
+        if (group < n_groups) {         // 16 lanes decide alike
+            unsigned int q[FMT == kMxFp4 ? 1 : 2];
+            const unsigned int word = mx_quantize8<FMT>(f[u], q);
+            store_group<FMT>(values, scales, group, lane16, q, word);
+        }
+    }
 }
 
-template <typename T, int FMT, bool VEC>
+// The same the other way.  16-bit results: eight neighbouring elements a lane, 16 bytes.  fp32: twice four, 64 elements
+// apart, so that 16 lanes write 256 bytes in a row each time.
+template <typename T, int FMT, bool VEC, int U>
 __global__ __launch_bounds__(kThreads) void mx_dequantize_kernel(const unsigned char* __restrict__ values,
                                                                  const unsigned char* __restrict__ scales, unsigned int n_groups,
                                                                  unsigned int row_groups, int d, long long ld, T* __restrict__ out) {
-    const unsigned int group = blockIdx.x * (kThreads / 16) + threadIdx.x / 16;
-    if (group >= n_groups) return;
+    constexpr int kBytes = mx_bytes<FMT>(128), P = sizeof(T) / 2;      // element bytes of a group; pieces a lane
+    const unsigned int first = blockIdx.x * (kThreads / 16 * U) + threadIdx.x / 16;
     const int lane16 = threadIdx.x & 15;
-    const unsigned int row = group / row_groups;
-    const int col = (int)(group - row * row_groups) * 128 + lane16 * 8;
-    if (col >= d) return;
-    unsigned int q[FMT == kMxFp4 ? 1 : 2];
-    if constexpr (FMT == kMxFp4) {
-        q[0] = reinterpret_cast<const unsigned int*>(values)[(long long)group * 16 + lane16];
-    } else {
-        const uint2 w = reinterpret_cast<const uint2*>(values)[(long long)group * 16 + lane16];
-        q[0] = w.x;
-        q[1] = w.y;
+    unsigned int q[U][2], word[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+        const unsigned int group = first + u * (kThreads / 16);
+        if (group >= n_groups) continue;
+        const unsigned char* v = values + (long long)group * kBytes;
+        word[u] = reinterpret_cast<const unsigned int*>(scales)[group];
+        if constexpr (P == 1 && FMT == kMxFp4) q[u][0] = reinterpret_cast<const unsigned int*>(v)[lane16];
+        if constexpr (P == 1 && FMT == kMxFp8) {
+            const uint2 w = reinterpret_cast<const uint2*>(v)[lane16];
+            q[u][0] = w.x;
+            q[u][1] = w.y;
+        }
+        if constexpr (P == 2) {
+            if constexpr (FMT == kMxFp4) {
+                q[u][0] = reinterpret_cast<const unsigned short*>(v)[lane16];
+                q[u][1] = reinterpret_cast<const unsigned short*>(v)[16 + lane16];
+            } else {
+                q[u][0] = reinterpret_cast<const unsigned int*>(v)[lane16];
+                q[u][1] = reinterpret_cast<const unsigned int*>(v)[16 + lane16];
+            }
+        }
     }
-    float f[8];
-    mx_dequantize8<FMT>(q, reinterpret_cast<const unsigned int*>(scales)[group], f);
-    T* p = out + (long long)row * ld + col;
-    if (VEC) store8<T>(p, f);
-    else store_some<T>(p, d - col, f);
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+        const unsigned int group = first + u * (kThreads / 16), row = group / row_groups;
+        if (group >= n_groups) continue;
+        const int col0 = (int)(group - row * row_groups) * 128;
+        T* o = out + (long long)row * ld;
+        if constexpr (P == 1) {
+            const int col = col0 + lane16 * 8;
+            const float s = mx_scale((word[u] >> (8 * (lane16 / 4))) & 255u);
+            float f[8];
+            mx_decode4<FMT>(FMT == kMxFp4 ? q[u][0] & 0xffffu : q[u][0], s, f);
+            mx_decode4<FMT>(FMT == kMxFp4 ? q[u][0] >> 16 : q[u][1], s, f + 4);
+            if (VEC && col < d) store8<T>(o + col, f);
+            else store_some<T>(o + col, d - col, f);
+        } else {
+#pragma unroll
+            for (int p = 0; p < 2; ++p) {
+                const int col = col0 + p * 64 + lane16 * 4;
+                float f[8];
+                mx_decode4<FMT>(q[u][p], mx_scale((word[u] >> (8 * (2 * p + lane16 / 8))) & 255u), f);
+                if (VEC && col < d) *reinterpret_cast<f32x4*>(o + col) = f32x4{f[0], f[1], f[2], f[3]};
+                else store_some<T>(o + col, d - col < 4 ? d - col : 4, f);
+            }
+        }
+    }
 }
 
 // y = h / sqrt(mean(h^2) + eps) * weight, h = x + residual, one workgroup of NT
@@ -148,28 +191,41 @@ __global__ __launch_bounds__(NT) void rms_norm_mx_kernel(const T* __restrict__ x
     }
 }
 
+// Groups a thread takes in turn, from where that still gives every CU several workgroups: half a million workgroups of
+// one group a thread take longer to start than to run, but a thread's accesses should stay near 64 bytes (measured, us,
+// one / two / four groups: a million rows of 1024, bf16 to 4 bits 528 / 480-500 / 480-500, back 480 / 428 / 416; 1000 wide,
+// bf16 to 8 bits 520 / 503 / 544, back 523 / 506 / 512; half a million of 1024, fp32 to 4 bits 385 / 400 / 412, back 395 / 402 / 420).
+template <typename T, int FMT> constexpr int kTurns = sizeof(T) == 4 ? 1 : FMT == kMxFp4 ? 4 : 2;
+constexpr unsigned int kTurnsFrom = 65536;
+
 template <typename T, int FMT>
 hipError_t quantize_typed(const void* x, long long n, int d, long long ld, void* values, void* scales, hipStream_t stream) {
     const unsigned int row_groups = mx_padded(d) / 128, n_groups = (unsigned int)(n * row_groups);
     const bool vec = d % 8 == 0 && (ld * sizeof(T)) % 16 == 0 && reinterpret_cast<uintptr_t>(x) % 16 == 0;
-    const dim3 grid((n_groups + kThreads / 16 - 1) / (kThreads / 16));
     const T* p = static_cast<const T*>(x);
     unsigned char *v = static_cast<unsigned char*>(values), *s = static_cast<unsigned char*>(scales);
-    if (vec) hipLaunchKernelGGL((mx_quantize_kernel<T, FMT, true>), grid, dim3(kThreads), 0, stream, p, n_groups, row_groups, d, ld, v, s);
-    else hipLaunchKernelGGL((mx_quantize_kernel<T, FMT, false>), grid, dim3(kThreads), 0, stream, p, n_groups, row_groups, d, ld, v, s);
-    return hipGetLastError();
+    const auto go = [&](auto kernel, unsigned int per_block) {
+        hipLaunchKernelGGL(kernel, dim3((n_groups + per_block - 1) / per_block), dim3(kThreads), 0, stream, p, n_groups, row_groups, d, ld, v, s);
+        return hipGetLastError();
+    };
+    constexpr int U = kTurns<T, FMT>;
+    if (n_groups < kTurnsFrom) return vec ? go(mx_quantize_kernel<T, FMT, true, 1>, kThreads / 16) : go(mx_quantize_kernel<T, FMT, false, 1>, kThreads / 16);
+    return vec ? go(mx_quantize_kernel<T, FMT, true, U>, kThreads / 16 * U) : go(mx_quantize_kernel<T, FMT, false, U>, kThreads / 16 * U);
 }
 
 template <typename T, int FMT>
 hipError_t dequantize_typed(const void* values, const void* scales, long long n, int d, void* out, long long ld, hipStream_t stream) {
     const unsigned int row_groups = mx_padded(d) / 128, n_groups = (unsigned int)(n * row_groups);
     const bool vec = d % 8 == 0 && (ld * sizeof(T)) % 16 == 0 && reinterpret_cast<uintptr_t>(out) % 16 == 0;
-    const dim3 grid((n_groups + kThreads / 16 - 1) / (kThreads / 16));
     const unsigned char *v = static_cast<const unsigned char*>(values), *s = static_cast<const unsigned char*>(scales);
     T* p = static_cast<T*>(out);
-    if (vec) hipLaunchKernelGGL((mx_dequantize_kernel<T, FMT, true>), grid, dim3(kThreads), 0, stream, v, s, n_groups, row_groups, d, ld, p);
-    else hipLaunchKernelGGL((mx_dequantize_kernel<T, FMT, false>), grid, dim3(kThreads), 0, stream, v, s, n_groups, row_groups, d, ld, p);
-    return hipGetLastError();
+    const auto go = [&](auto kernel, unsigned int per_block) {
+        hipLaunchKernelGGL(kernel, dim3((n_groups + per_block - 1) / per_block), dim3(kThreads), 0, stream, v, s, n_groups, row_groups, d, ld, p);
+        return hipGetLastError();
+    };
+    constexpr int U = kTurns<T, FMT>;
+    if (n_groups < kTurnsFrom) return vec ? go(mx_dequantize_kernel<T, FMT, true, 1>, kThreads / 16) : go(mx_dequantize_kernel<T, FMT, false, 1>, kThreads / 16);
+    return vec ? go(mx_dequantize_kernel<T, FMT, true, U>, kThreads / 16 * U) : go(mx_dequantize_kernel<T, FMT, false, U>, kThreads / 16 * U);
 }
 
 struct NormArgs {

@@ -43,7 +43,7 @@ def check_quantized(got, x64, fmt):
 
 # ---- rows to microscaled floating point and back ---------------------------------
 
-SHAPES = [(1, 1), (1, 32), (2, 31), (3, 33), (5, 127), (4, 128), (7, 129), (34, 1000), (17, 1024), (3, 4100), (1000, 8)]
+SHAPES = [(1, 1), (1, 32), (2, 31), (3, 33), (5, 127), (4, 128), (7, 129), (34, 1000), (17, 1024), (3, 4100), (1000, 8), (66001, 9), (8200, 1032)]
 
 
 @pytest.mark.parametrize("fmt", ["mxfp4", "mxfp8"])
