@@ -152,6 +152,16 @@ int main() {
     }
     EXPECT(mtr_merge_topk_device(nullptr, nullptr, 1, 0, 0, 1, 1, 1, nullptr, nullptr, 0, nullptr) == MTR_ERR_INVALID);
     EXPECT(mtr_pool_normalize(nullptr, 0, nullptr, 1, 1, 1, nullptr, 0, nullptr) == MTR_ERR_INVALID);
+    // the scoring head's operators
+    EXPECT(mtr_mx_quantize(nullptr, MTR_F32, 1, 8, 8, MTR_MX_FP4, nullptr, nullptr, 0, nullptr) == MTR_ERR_INVALID);
+    EXPECT(mtr_mx_quantize(nullptr, MTR_F32, 0, 8, 8, MTR_MX_FP4, nullptr, nullptr, 0, nullptr) == MTR_OK);
+    EXPECT(mtr_mx_dequantize(nullptr, nullptr, MTR_MX_FP8, 1, 8, nullptr, MTR_F32, 8, 0, nullptr) == MTR_ERR_INVALID);
+    EXPECT(mtr_rms_norm_mx(nullptr, nullptr, nullptr, MTR_BF16, MTR_BF16, 1, 8, 8, 0, 1e-6f, MTR_MX_FP8, nullptr, nullptr, nullptr, 0, nullptr) ==
+           MTR_ERR_INVALID);
+    EXPECT(mtr_mx_matmul(nullptr, nullptr, MTR_MX_FP8, 1, nullptr, nullptr, 1, 8, nullptr, MTR_F32, 1, nullptr, 0, 0, nullptr) == MTR_ERR_INVALID);
+    EXPECT(mtr_mx_matmul_workspace(1, 1 << 20, 4096) == 0 && mtr_mx_matmul_workspace(4096, 4096, 4096) == (int64_t)8192 * 32 * 4);
+    EXPECT(mtr_token_logprobs(nullptr, MTR_F32, 1, 8, 8, nullptr, 0, 0, nullptr, nullptr, nullptr, nullptr, nullptr, 0, 0, nullptr) == MTR_ERR_INVALID);
+    EXPECT(mtr_token_logprobs_workspace(1, 1000, 5) == 0 && mtr_token_logprobs_workspace(1, 1 << 20, 5) > 0);
     EXPECT(mtr_comm_create(nullptr, 0, 1, 0, nullptr) == MTR_ERR_INVALID);
     mtr_comm_t* comm = nullptr;
     EXPECT(mtr_comm_create(nullptr, 0, 1, 0, &comm) == MTR_ERR_INVALID && comm == nullptr);

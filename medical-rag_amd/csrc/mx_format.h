@@ -96,17 +96,17 @@ __device__ __forceinline__ unsigned int mx_quantize8(const float (&f)[8], unsign
     s = s < -127 ? -127 : s;
     const float r = __uint_as_float(a) * __uint_as_float((unsigned int)(127 - s) << 23);
     s += (FMT == kMxFp4 ? r >= 7.f : r > 464.f) ? 1 : 0;
-    const float inv = bad ? 0.f : __uint_as_float((unsigned int)(127 - s) << 23);
+    const float inv = __uint_as_float((unsigned int)(127 - s) << 23);      // of a block that holds no number: anything, its elements are cleared
     float y[8];
 #pragma unroll
-    for (int i = 0; i < 8; ++i) y[i] = bad ? 0.f : f[i] * inv;
+    for (int i = 0; i < 8; ++i) y[i] = f[i] * inv;
     if constexpr (FMT == kMxFp4) {      // rounds to nearest even and saturates at 6
         unsigned int w = 0;
         w = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(w, y[0], y[1], 1.f, 0);
         w = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(w, y[2], y[3], 1.f, 1);
         w = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(w, y[4], y[5], 1.f, 2);
         w = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(w, y[6], y[7], 1.f, 3);
-        q[0] = w;
+        q[0] = bad ? 0u : w;
     } else {
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
@@ -116,7 +116,7 @@ __device__ __forceinline__ unsigned int mx_quantize8(const float (&f)[8], unsign
             for (int i = 0; i < 4; ++i) c[i] = __builtin_amdgcn_fmed3f(y[4 * h + i], -448.f, 448.f);   // at most 464 comes in
             w = __builtin_amdgcn_cvt_pk_fp8_f32(c[0], c[1], w, false);
             w = __builtin_amdgcn_cvt_pk_fp8_f32(c[2], c[3], w, true);
-            q[h] = (unsigned int)w;
+            q[h] = bad ? 0u : (unsigned int)w;
         }
     }
     const unsigned int quad = (threadIdx.x >> 2) & 3;

@@ -518,13 +518,14 @@ def test_the_head_as_a_run(sc):
         assert (np.abs(np.take_along_axis(want, ids.cpu().numpy(), 1) - best) <= 2 * slack[:, None]).all()
 
 
-def test_captured_and_replayed(sc):
+@pytest.mark.parametrize("n", [3, 300])
+def test_captured_and_replayed(sc, n):
     """The head in a HIP graph, replayed on new inputs with eager work in between."""
     import torch
-    n, d, v = 3, 300, 20000
+    d, v = 300, 20000
     x, res, w = rows(n, d, "bfloat16", seed=1), rows(n, d, "bfloat16", seed=2), rows(1, d, "bfloat16", seed=3)[0]
     vocab = sc.mx_quantize(rows(v, d, "bfloat16", seed=4, spread=0.1), "mxfp4")
-    tokens = torch.tensor([[5], [6], [7]], device="cuda")
+    tokens = torch.arange(n, device="cuda")[:, None].contiguous()
     side = torch.cuda.Stream()
     side.wait_stream(torch.cuda.current_stream())
     with torch.cuda.stream(side):
@@ -547,11 +548,12 @@ def test_captured_and_replayed(sc):
                 assert torch.equal(a, b)
 
 
-def test_on_two_streams_at_once_and_twice_the_same(sc):
+@pytest.mark.parametrize("n", [1, 64, 130])
+def test_on_two_streams_at_once_and_twice_the_same(sc, n):
     import torch
-    x, res, w = rows(64, 1024, "bfloat16", seed=1), rows(64, 1024, "bfloat16", seed=2), rows(1, 1024, "bfloat16", seed=3)[0]
+    x, res, w = rows(n, 1024, "bfloat16", seed=1), rows(n, 1024, "bfloat16", seed=2), rows(1, 1024, "bfloat16", seed=3)[0]
     vocab = sc.mx_quantize(rows(30000, 1024, "bfloat16", seed=4, spread=0.1), "mxfp4")
-    tokens = torch.randint(0, 30000, (64, 1), generator=torch.Generator().manual_seed(5)).cuda()
+    tokens = torch.randint(0, 30000, (n, 1), generator=torch.Generator().manual_seed(5)).cuda()
     want = head(sc, x, res, w, vocab, tokens)
     torch.cuda.synchronize()
     streams = [torch.cuda.Stream(), torch.cuda.Stream()]
