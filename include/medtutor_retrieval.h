@@ -282,7 +282,8 @@ int mtr_pool_normalize(const void* dev_hidden, int32_t dtype, const int64_t* dev
  *           block that held a NaN or infinity and reads back as NaN; on 4 bytes
  * The scale is the smallest 2^s (s >= -127) under which the block's largest
  * magnitude rounds to the largest element (6 and 448) or less; elements are
- * rounded to nearest, ties to even. */
+ * rounded to nearest, ties to even.  Results never overlap operands.  n, and
+ * n times the MTR_MX_PAD wide pieces of a row, stay below 2^31. */
 enum { MTR_MX_FP4 = 0, MTR_MX_FP8 = 1 };
 #define MTR_MX_BLOCK 32
 #define MTR_MX_PAD 128
@@ -291,7 +292,7 @@ int mtr_mx_quantize(const void* dev_x, int32_t dtype, int64_t n, int32_t d, int6
 int mtr_mx_dequantize(const void* dev_values, const void* dev_scales, int32_t format, int64_t n, int32_t d,
                       void* dev_out, int32_t dtype, int64_t ld, int32_t device_id, void* stream);
 /* h = x + residual, rounded to their type and written to dev_residual_out (dense
- * rows; it may be the residual's own memory when that is dense); then
+ * rows); then
  * h / sqrt(mean(h^2) + eps) * weight as microscaled rows.  dev_residual and
  * dev_residual_out both NULL: h = x.  weight: d elements of the rows' type or
  * fp32.  d <= MTR_RMS_NORM_MAX_WIDTH. */
@@ -301,8 +302,10 @@ int mtr_rms_norm_mx(const void* dev_x, const void* dev_residual, const void* dev
                     int32_t format, void* dev_residual_out, void* dev_values, void* dev_scales,
                     int32_t device_id, void* stream);
 /* out[m][n] = A (m rows of d, either format) times the transpose of B (n rows of d,
- * MTR_MX_FP4), MTR_F32 or MTR_BF16.  Workspace: mtr_mx_matmul_workspace bytes on 4
- * bytes, the caller's, not shared by calls that may overlap. */
+ * MTR_MX_FP4), MTR_F32 or MTR_BF16; m and n up to MTR_MX_MATMUL_MAX_ROWS.
+ * Workspace: mtr_mx_matmul_workspace bytes on 4 bytes, the caller's, not shared by
+ * calls that may overlap. */
+#define MTR_MX_MATMUL_MAX_ROWS 536870912
 int64_t mtr_mx_matmul_workspace(int64_t m, int64_t n, int32_t d);
 int mtr_mx_matmul(const void* dev_a_values, const void* dev_a_scales, int32_t a_format, int64_t m,
                   const void* dev_b_values, const void* dev_b_scales, int64_t n, int32_t d, void* dev_out,
@@ -314,7 +317,7 @@ int mtr_mx_matmul(const void* dev_a_values, const void* dev_a_scales, int32_t a_
  * -inf are excluded: log probability -inf, never an alternative; slots beyond the
  * tokens that are left hold id -1 and -inf.  A row with nothing left has entropy 0.
  * A row that holds a NaN or +inf has NaN everywhere and ids -1.  A negative token
- * is padding (0), one >= v gives NaN.  Workspace: mtr_token_logprobs_workspace
+ * is padding (0), one >= v gives NaN.  n < 2^21, v < 2^31.  Workspace: mtr_token_logprobs_workspace
  * bytes on 8 bytes, the caller's, not shared by calls that may overlap. */
 #define MTR_MAX_ALTERNATIVES 64
 int64_t mtr_token_logprobs_workspace(int64_t n, int64_t v, int32_t top_k);

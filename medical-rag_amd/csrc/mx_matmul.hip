@@ -624,7 +624,7 @@ template <int FA, bool EXACT, int WM, int STAGES, int PER_CU, typename TO> hipEr
     if (e != hipSuccess) return e;
     p.m_tiles = (int)((p.m + S::M - 1) / S::M);
     const long long tiles = p.m_tiles * ((p.n + kTileN - 1) / kTileN);
-    if (tiles > 0x7fffffff) return hipErrorInvalidValue;
+    if (tiles > 0x7fffff) return hipErrorInvalidValue;      // a launch counts its threads in 32 bits
     hipLaunchKernelGGL((mx_matmul_tile_kernel<FA, EXACT, WM, STAGES, PER_CU, TO>), dim3((unsigned int)tiles), dim3(kTileThreads), lds, stream, p);
     return hipGetLastError();
 }
@@ -668,6 +668,7 @@ hipError_t launch_mx_matmul(const void* a_values, const void* a_scales, int a_fo
         const Turn ta{static_cast<const unsigned int*>(a_scales), m, up(m, 256), as}, tb{static_cast<const unsigned int*>(b_scales), n, up(n, 256), bs};
         const dim3 turn_grid((unsigned int)((up(m, 256) + up(n, 256)) / 64), (unsigned int)((groups + 31) / 32));
         hipLaunchKernelGGL(turn_scales_kernel, turn_grid, dim3(256), 0, stream, ta, tb, groups);
+        if (const hipError_t e = hipGetLastError(); e != hipSuccess) return e;
         const TileArgs p{a, b, as, bs, m, n, up(m, 256), up(n, 256), groups, 0, out, ld_out, whole, past};
         if (a_format == kMxFp4) return out_dtype == 0 ? tiles_4bit<float>(p, stream) : tiles_4bit<bf16_t>(p, stream);
         return out_dtype == 0 ? tiles_8bit<true, float>(p, stream) : tiles_8bit<false, bf16_t>(p, stream);

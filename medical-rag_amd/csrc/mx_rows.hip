@@ -270,41 +270,87 @@ template <typename T> hipError_t norm_format(const NormArgs& a, int format, hipS
 
 }  // namespace
 
-hipError_t launch_mx_quantize(const void* x, int dtype, long long n, int d, long long ld, int format, void* values, void* scales,
-                              hipStream_t stream) {
-#define MTR_BY_FORMAT(T) format == kMxFp4 ? quantize_typed<T, kMxFp4>(x, n, d, ld, values, scales, stream) : quantize_typed<T, kMxFp8>(x, n, d, ld, values, scales, stream)
+namespace {
+
+template <int FMT> hipError_t quantize_piece(const void* x, int dtype, long long n, int d, long long ld, void* values, void* scales,
+                                             hipStream_t stream) {
     switch (dtype) {
-        case 0: return MTR_BY_FORMAT(float);
-        case 2: return MTR_BY_FORMAT(bf16_t);
-        case 3: return MTR_BY_FORMAT(_Float16);
+        case 0: return quantize_typed<float, FMT>(x, n, d, ld, values, scales, stream);
+        case 2: return quantize_typed<bf16_t, FMT>(x, n, d, ld, values, scales, stream);
+        case 3: return quantize_typed<_Float16, FMT>(x, n, d, ld, values, scales, stream);
         default: return hipErrorInvalidValue;
     }
-#undef MTR_BY_FORMAT
+}
+
+template <int FMT> hipError_t dequantize_piece(const void* values, const void* scales, long long n, int d, void* out, int dtype, long long ld,
+                                               hipStream_t stream) {
+    switch (dtype) {
+        case 0: return dequantize_typed<float, FMT>(values, scales, n, d, out, ld, stream);
+        case 2: return dequantize_typed<bf16_t, FMT>(values, scales, n, d, out, ld, stream);
+        case 3: return dequantize_typed<_Float16, FMT>(values, scales, n, d, out, ld, stream);
+        default: return hipErrorInvalidValue;
+    }
+}
+
+// A launch counts its threads in 32 bits: matrices of more take several.
+template <typename F> hipError_t in_pieces(long long n, long long rows_a_launch, F&& launch) {
+    for (long long r = 0; r < n; r += rows_a_launch) {
+        const hipError_t e = launch(r, n - r < rows_a_launch ? n - r : rows_a_launch);
+        if (e != hipSuccess) return e;
+    }
+    return hipSuccess;
+}
+
+struct RowBytes {       // of a stored row
+    long long values, scales, a_launch;     // a_launch: rows whose groups, 16 threads each, are 2^31 threads
+    RowBytes(int format, int d)
+        : values(format == kMxFp4 ? mx_padded(d) / 2 : mx_padded(d)), scales(mx_padded(d) / kMxBlock), a_launch((1 << 27) / (mx_padded(d) / 128)) {}
+};
+
+long long size_of(int dtype) { return dtype == 0 ? 4 : 2; }
+
+}  // namespace
+
+hipError_t launch_mx_quantize(const void* x, int dtype, long long n, int d, long long ld, int format, void* values, void* scales,
+                              hipStream_t stream) {
+    const RowBytes row(format, d);
+    return in_pieces(n, row.a_launch, [&](long long r, long long rows) {
+        const char* px = static_cast<const char*>(x) + r * ld * size_of(dtype);
+        char *pv = static_cast<char*>(values) + r * row.values, *ps = static_cast<char*>(scales) + r * row.scales;
+        return format == kMxFp4 ? quantize_piece<kMxFp4>(px, dtype, rows, d, ld, pv, ps, stream) : quantize_piece<kMxFp8>(px, dtype, rows, d, ld, pv, ps, stream);
+    });
 }
 
 hipError_t launch_mx_dequantize(const void* values, const void* scales, int format, long long n, int d, void* out, int dtype,
                                 long long ld, hipStream_t stream) {
-#define MTR_BY_FORMAT(T) format == kMxFp4 ? dequantize_typed<T, kMxFp4>(values, scales, n, d, out, ld, stream) : dequantize_typed<T, kMxFp8>(values, scales, n, d, out, ld, stream)
-    switch (dtype) {
-        case 0: return MTR_BY_FORMAT(float);
-        case 2: return MTR_BY_FORMAT(bf16_t);
-        case 3: return MTR_BY_FORMAT(_Float16);
-        default: return hipErrorInvalidValue;
-    }
-#undef MTR_BY_FORMAT
+    const RowBytes row(format, d);
+    return in_pieces(n, row.a_launch, [&](long long r, long long rows) {
+        char* po = static_cast<char*>(out) + r * ld * size_of(dtype);
+        const char *pv = static_cast<const char*>(values) + r * row.values, *ps = static_cast<const char*>(scales) + r * row.scales;
+        return format == kMxFp4 ? dequantize_piece<kMxFp4>(pv, ps, rows, d, po, dtype, ld, stream) : dequantize_piece<kMxFp8>(pv, ps, rows, d, po, dtype, ld, stream);
+    });
 }
 
 hipError_t launch_rms_norm_mx(const void* x, const void* residual, const void* weight, int dtype, int weight_dtype, long long n,
                               int d, long long ld_x, long long ld_residual, float eps, int format, void* residual_out,
                               void* values, void* scales, hipStream_t stream) {
     if (d > kRmsNormMaxWidth || (weight_dtype != dtype && weight_dtype != 0)) return hipErrorInvalidValue;
-    const NormArgs a{x, residual, weight, weight_dtype == 0, n, d, ld_x, ld_residual, eps, residual_out, values, scales};
-    switch (dtype) {
-        case 0: return norm_format<float>(a, format, stream);
-        case 2: return norm_format<bf16_t>(a, format, stream);
-        case 3: return norm_format<_Float16>(a, format, stream);
-        default: return hipErrorInvalidValue;
-    }
+    const RowBytes row(format, d);
+    const long long size = size_of(dtype);
+    return in_pieces(n, 1 << 21, [&](long long r, long long rows) {     // of 1024 threads at most
+        NormArgs a{static_cast<const char*>(x) + r * ld_x * size, residual, weight, weight_dtype == 0, rows, d, ld_x, ld_residual, eps, residual_out,
+                   static_cast<char*>(values) + r * row.values, static_cast<char*>(scales) + r * row.scales};
+        if (residual) {
+            a.residual = static_cast<const char*>(residual) + r * ld_residual * size;
+            a.residual_out = static_cast<char*>(residual_out) + r * d * size;
+        }
+        switch (dtype) {
+            case 0: return norm_format<float>(a, format, stream);
+            case 2: return norm_format<bf16_t>(a, format, stream);
+            case 3: return norm_format<_Float16>(a, format, stream);
+            default: return hipErrorInvalidValue;
+        }
+    });
 }
 
 }  // namespace mtr

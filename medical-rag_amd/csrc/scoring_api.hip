@@ -38,10 +38,11 @@ bool off(const void* p, uintptr_t bytes) { return reinterpret_cast<uintptr_t>(p)
 uintptr_t size_of(int32_t dtype) { return dtype == MTR_F32 ? 4 : 2; }
 
 constexpr int64_t kMost = 0x7fffffff;       // rows, row groups and workgroups are numbered in 31 bits
+constexpr int64_t kMostProduct = MTR_MX_MATMUL_MAX_ROWS;    // a launch counts its threads in 32 bits, four a row
 
 int check_rows(const char* what, int64_t n, int32_t d, const void* values, const void* scales, int32_t format) {
     if (!is_mx(format)) return set_error(MTR_ERR_INVALID, "%s: bad format %d", what, format);
-    if (n < 0 || d < 1 || d > kMost - MTR_MX_PAD || n * (mtr::mx_padded(d) / MTR_MX_PAD) > kMost || n > kMost)
+    if (n < 0 || n > kMost || d < 1 || d > kMost - MTR_MX_PAD || n * (mtr::mx_padded(d) / MTR_MX_PAD) > kMost)
         return set_error(MTR_ERR_INVALID, "%s: bad shape (n=%lld, d=%d)", what, (long long)n, d);
     if (n == 0) return MTR_OK;
     if (!values || !scales) return set_error(MTR_ERR_INVALID, "%s: NULL argument", what);
@@ -93,6 +94,8 @@ int mtr_rms_norm_mx(const void* dev_x, const void* dev_residual, const void* dev
     if (!dev_x || !dev_weight) return set_error(MTR_ERR_INVALID, "NULL argument");
     if (!dev_residual != !dev_residual_out)
         return set_error(MTR_ERR_INVALID, "a residual and the place for the updated one come together");
+    if (dev_residual && (dev_residual_out == dev_residual || dev_residual_out == dev_x))
+        return set_error(MTR_ERR_INVALID, "the updated residual wants memory of its own");
     const uintptr_t size = size_of(dtype);
     if (off(dev_x, size) || off(dev_weight, size_of(weight_dtype)) || off(dev_residual, size) || off(dev_residual_out, size) ||
         ld_x < 0 || ld_residual < 0)
@@ -105,7 +108,7 @@ int mtr_rms_norm_mx(const void* dev_x, const void* dev_residual, const void* dev
 }
 
 int64_t mtr_mx_matmul_workspace(int64_t m, int64_t n, int32_t d) {
-    if (m < 1 || n < 1 || d < 1 || d > kMost - MTR_MX_PAD || m > kMost || n > kMost) return 0;
+    if (m < 1 || n < 1 || d < 1 || d > kMost - MTR_MX_PAD || m > kMostProduct || n > kMostProduct) return 0;
     return mtr::mx_matmul_workspace(m, n, d);
 }
 
@@ -115,6 +118,7 @@ int mtr_mx_matmul(const void* dev_a_values, const void* dev_a_scales, int32_t a_
     if (out_dtype != MTR_F32 && out_dtype != MTR_BF16) return set_error(MTR_ERR_INVALID, "bad output dtype %d", out_dtype);
     if (int rc = check_rows("mtr_mx_matmul", m, d, dev_a_values, dev_a_scales, a_format)) return rc;
     if (int rc = check_rows("mtr_mx_matmul", n, d, dev_b_values, dev_b_scales, MTR_MX_FP4)) return rc;
+    if (m > kMostProduct || n > kMostProduct) return set_error(MTR_ERR_INVALID, "bad shape (m=%lld, n=%lld)", (long long)m, (long long)n);
     if (m == 0 || n == 0) return MTR_OK;
     if (!dev_out) return set_error(MTR_ERR_INVALID, "NULL argument");
     if (off(dev_out, size_of(out_dtype)) || (m > 1 && ld_out < n))

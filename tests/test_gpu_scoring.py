@@ -86,6 +86,24 @@ def test_quantize_extremes(sc, fmt):
     assert torch.isnan(back[11, :32]).all() and back[11, 63] == 3
 
 
+def test_more_rows_than_one_launch_counts(sc):
+    """2^32 threads and more: every row is written, the last ones too (all rows are one row)."""
+    import torch
+    for n, d in ((150_000_000, 200), (300_000_000, 2)):     # 2 and 1 groups of 128 a row, 16 threads each
+        x = torch.linspace(-3, 5, d, device="cuda")[None]
+        got, one = sc.mx_quantize(x.expand(n, d)), sc.mx_quantize(x)
+        words, want = got.values.view(torch.int64), one.values.view(torch.int64)
+        step = 1 << 24
+        assert all((words[lo:lo + step] == want).all() for lo in range(0, n, step))
+        assert all((got.scales[lo:lo + step] == one.scales).all() for lo in range(0, n, step))
+        if d == 2:
+            out = torch.full((n, d), 7.0, dtype=torch.bfloat16, device="cuda")
+            sc.mx_dequantize(got, out=out)
+            back = sc.mx_dequantize(one)
+            assert all((out[lo:lo + step] == back).all() for lo in range(0, n, step))
+        del got, words
+
+
 @pytest.mark.parametrize("dtype", DTYPES)
 @pytest.mark.parametrize("fmt", ["mxfp4", "mxfp8"])
 def test_dequantize_rounds_once(sc, dtype, fmt):
@@ -457,6 +475,17 @@ def test_logits_strided_misaligned_and_far_apart(sc):
     far.copy_(logits_of(3, 5000, "bfloat16", seed=3))
     check_logprobs(sc, far, torch.tensor([4999, 0, 17], device="cuda"), 3)
     assert sc.token_logprobs(far[:0], far[:0, 0].long(), 3).top_ids.shape == (0, 3)
+
+
+def test_rms_norm_more_rows_than_one_launch_counts(sc):
+    import torch
+    n, d = 17_000_000, 513
+    x, res, w = rows(1, d, "bfloat16", seed=1), rows(1, d, "bfloat16", seed=2), rows(1, d, "bfloat16", seed=3)[0]
+    got, h = sc.rms_norm_mx(x.expand(n, d), w, residual=res.expand(n, d), format="mxfp4")
+    one, h1 = sc.rms_norm_mx(x, w, residual=res, format="mxfp4")
+    words, want, step = got.values.view(torch.int64), one.values.view(torch.int64), 1 << 22
+    for lo in range(0, n, step):
+        assert (words[lo:lo + step] == want).all() and (got.scales[lo:lo + step] == one.scales).all() and (h[lo:lo + step] == h1).all()
 
 
 # ---- how they are called ---------------------------------------------------------------

@@ -80,6 +80,7 @@ def test_c_refusals_come_before_any_hip_call():
     refuses(q(d=2 ** 31 - 1), "shape")
     refuses(q(n=2 ** 31, d=8), "shape")
     refuses(q(n=2 ** 24, d=2 ** 20), "shape")
+    refuses(q(n=2 ** 62, d=512), "shape")
     refuses(q(x=None), "NULL")
     refuses(q(v=None), "NULL")
     refuses(q(s=None), "NULL")
@@ -104,6 +105,8 @@ def test_c_refusals_come_before_any_hip_call():
     refuses(norm(eps=float("nan")), "eps")
     refuses(norm(r=at), "together")
     refuses(norm(ro=at), "together")
+    refuses(norm(r=at, ro=at + 1024, x=at + 1024), "of its own")
+    refuses(norm(r=at, ro=at, x=at + 1024), "of its own")
     refuses(norm(w=None), "NULL")
     refuses(norm(x=at + 1), "address")
     refuses(norm(ldx=-8), "stride")
@@ -118,6 +121,9 @@ def test_c_refusals_come_before_any_hip_call():
     refuses(mm(o=None), "NULL")
     refuses(mm(ld=1), "stride")
     refuses(mm(m=-1), "shape")
+    refuses(mm(n=2 ** 29 + 1, ld=2 ** 30), "shape")
+    refuses(mm(m=2 ** 29 + 1), "shape")
+    assert lib.mtr_mx_matmul_workspace(4, 2 ** 29 + 1, 8) == 0
     assert lib.mtr_mx_matmul_workspace(3000, 5000, 1000) > 0 and lib.mtr_mx_matmul_workspace(0, 5, 5) == 0
     refuses(mm(m=3000, n=5000, d=1000, ld=5000), "workspace")
     refuses(mm(m=3000, n=5000, d=1000, ld=5000, w=at, wb=64), "workspace")
