@@ -28,6 +28,7 @@ __all__ = ["MxRows", "TokenLogprobs", "mx_quantize", "mx_dequantize", "rms_norm_
 
 FORMATS = {"mxfp4": _native.MTR_MX_FP4, "mxfp8": _native.MTR_MX_FP8}
 BLOCK, PAD = _native.MTR_MX_BLOCK, _native.MTR_MX_PAD
+MOST = (1 << 31) - 1        # what the library's 32-bit numbers hold: ctypes would cut off the rest without a word
 
 TokenLogprobs = namedtuple("TokenLogprobs", "logprobs entropy top_ids top_logprobs")
 TokenLogprobs.__doc__ = """What token_logprobs returns: logprobs (n, g) and entropy (n,) float32, top_ids (n, top_k)
@@ -55,6 +56,16 @@ def _rows(x, what):
     return x if x.stride(1) == 1 or x.shape[1] < 2 else x.contiguous()
 
 
+def _into(out, what):
+    """Checks `out` of an operator without a backward pass, and tells autograd that it is overwritten."""
+    if not isinstance(out, torch.Tensor) or not out.is_cuda:
+        raise ValueError(f"{what}: out must be a GPU tensor")
+    if out.requires_grad and torch.is_grad_enabled():
+        raise ValueError(f"{what} has no backward pass: its out must not record one")
+    if not out.is_inference():
+        torch.autograd.graph.increment_version(out)
+
+
 def _width(d, format):
     """(element bytes, scale bytes) of a stored row."""
     padded = (d + PAD - 1) // PAD * PAD
@@ -72,8 +83,8 @@ class MxRows:
     def __init__(self, values, scales, d: int, format: str = "mxfp4"):
         if format not in FORMATS:
             raise ValueError(f"format must be one of {sorted(FORMATS)}")
-        if d < 1:
-            raise ValueError("rows need at least one element")
+        if not 1 <= d <= MOST:
+            raise ValueError(f"rows of {d} elements: at least one, at most {MOST}")
         for t in (values, scales):
             if not isinstance(t, torch.Tensor) or not t.is_cuda or t.dtype != torch.uint8 or t.dim() != 2 or not t.is_contiguous():
                 raise ValueError("MxRows wants contiguous 2-D uint8 GPU tensors")
@@ -92,8 +103,8 @@ class MxRows:
         """Room for n rows, values and scales in one allocation."""
         if format not in FORMATS:
             raise ValueError(f"format must be one of {sorted(FORMATS)}")
-        if d < 1:
-            raise ValueError("rows need at least one element")
+        if not 1 <= d <= MOST:
+            raise ValueError(f"rows of {d} elements: at least one, at most {MOST}")
         width, blocks = _width(d, format)
         rows = cls.__new__(cls)
         both = torch.empty_strided((n * (width + blocks),), (1,), dtype=torch.uint8, device=device)
@@ -128,6 +139,9 @@ class MxRows:
         """Rows [lo, hi) as a view."""
         return MxRows(self.values[lo:hi], self.scales[lo:hi], self.d, self.format)
 
+    def __reduce__(self):       # copies and pickles hold their own tensors' addresses
+        return MxRows, (self.values, self.scales, self.d, self.format)
+
     def __repr__(self):
         return f"MxRows({len(self)} x {self.d}, {self.format}, {self.device})"
 
@@ -160,6 +174,7 @@ def mx_dequantize(rows: MxRows, dtype=None, out=None):
         code = _code(dtype, "mx_dequantize")
         out = torch.empty_strided((n, d), (d, 1), dtype=dtype, device=device)
     else:
+        _into(out, "mx_dequantize")
         code = _code(out.dtype, "mx_dequantize")
         if out.shape != (n, d) or out.device != device or (d > 1 and out.stride(1) != 1) or (dtype is not None and dtype != out.dtype):
             raise ValueError("out must be a (n, d) tensor of the dtype on the rows' GPU, its rows dense")
@@ -227,8 +242,10 @@ def mx_matmul(a: MxRows, b: MxRows, dtype=None, out=None):
         dtype = dtype or torch.float32
         line = 32 if dtype == torch.float32 else 64
         out = torch.empty_strided((m, n), (n if n < 1024 else (n + line - 1) // line * line, 1), dtype=dtype, device=device)
-    elif out.shape != (m, n) or out.device != device or (n > 1 and out.stride(1) != 1) or (dtype is not None and dtype != out.dtype):
-        raise ValueError("out must be a (m, n) tensor of the dtype on the operands' GPU, its rows dense")
+    else:
+        _into(out, "mx_matmul")
+        if out.shape != (m, n) or out.device != device or (n > 1 and out.stride(1) != 1) or (dtype is not None and dtype != out.dtype):
+            raise ValueError("out must be a (m, n) tensor of the dtype on the operands' GPU, its rows dense")
     if out.dtype not in (torch.float32, torch.bfloat16):
         raise TypeError(f"mx_matmul: unsupported dtype {out.dtype}")
     lib = _native.lib()
@@ -266,6 +283,8 @@ def token_logprobs(logits, tokens=None, top_k: int = 0) -> TokenLogprobs:
             raise ValueError(f"token_logprobs wants ({n},) or ({n}, g) tokens, got {tuple(tokens.shape)}")
         tokens = tokens.contiguous()
         g = tokens.shape[1]
+        if g > MOST:
+            raise ValueError(f"{g} tokens a row: at most {MOST}")
     if not 0 <= top_k <= _native.MTR_MAX_ALTERNATIVES:
         raise ValueError(f"top_k must be in [0, {_native.MTR_MAX_ALTERNATIVES}]")
     lib = _native.lib()

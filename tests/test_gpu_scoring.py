@@ -520,6 +520,41 @@ def test_refusals(sc):
         sc.mx_quantize(x.clone().requires_grad_())
 
 
+def test_copies_have_their_own_memory(sc):
+    """deepcopy and pickle of rows made in one allocation, of given tensors and of a view."""
+    import copy
+    import pickle
+
+    import torch
+    made = sc.mx_quantize(rows(5, 200, "float32"), "mxfp8")
+    given = sc.MxRows(made.values.clone(), made.scales.clone(), 200, "mxfp8")
+    for r in (made, given, made.rows(1, 4)):
+        want = sc.mx_dequantize(r, torch.float32)
+        copies = [copy.deepcopy(r), pickle.loads(pickle.dumps(r))]
+        kept = r.values.clone()
+        r.values.zero_()
+        for c in copies:
+            assert torch.equal(sc.mx_dequantize(c, torch.float32), want) and (len(c), c.d, c.format) == (len(r), 200, "mxfp8")
+        r.values.copy_(kept)
+
+
+def test_out_is_seen_by_autograd(sc):
+    """A tensor that a recorded operation needs is overwritten: its backward pass says so; one that records is refused."""
+    import torch
+    x = torch.ones(4, 64, device="cuda")
+    q4, q8 = sc.mx_quantize(x), sc.mx_quantize(x, "mxfp8")
+    for call, shape in ((lambda o: sc.mx_dequantize(q4, out=o), (4, 64)), (lambda o: sc.mx_matmul(q8, q4, out=o), (4, 4))):
+        out, w = torch.zeros(shape, device="cuda"), torch.ones(shape, device="cuda", requires_grad=True)
+        y = (out * w).sum()
+        assert call(out) is out and bool((out != 0).all())
+        with pytest.raises(RuntimeError):
+            y.backward()
+        with pytest.raises(ValueError):
+            call(w)
+        with pytest.raises(ValueError):
+            call(out.cpu())
+
+
 def head(sc, x, res, w, vocab, tokens):
     y, h = sc.rms_norm_mx(x, w, 1e-6, res)
     return (h,) + tuple(sc.token_logprobs(sc.mx_matmul(y, vocab), tokens, 5))

@@ -162,6 +162,9 @@ def test_python_refuses_what_is_not_on_a_gpu():
         scoring.MxRows(None, None, 8, "int4")
     with pytest.raises(ValueError):
         scoring.MxRows(None, None, 0)
+    for d in (2 ** 31, 2 ** 32 + 5):        # would reach the library as another width
+        with pytest.raises(ValueError):
+            scoring.MxRows.empty(1, d, "mxfp4", "cpu")
 
 
 def test_constants_match_the_header():
