@@ -16,6 +16,7 @@ through them.  There is no CPU form.
 from __future__ import annotations
 
 import logging
+import threading
 
 import numpy as np
 import torch
@@ -74,8 +75,9 @@ class ScoringHead:
         step = max(1, (2 << 30) // (4 * len(self.vocabulary)))
         if len(hidden) <= step:
             return scoring.token_logprobs(self.logits(hidden, residual), tokens, top_k)
-        parts = [scoring.token_logprobs(self.logits(hidden[lo:lo + step], None if residual is None else residual[lo:lo + step]),
-                                        tokens[lo:lo + step], top_k) for lo in range(0, len(hidden), step)]
+        cut = lambda t, lo: None if t is None else t[lo:lo + step]  # noqa: E731
+        parts = [scoring.token_logprobs(self.logits(cut(hidden, lo), cut(residual, lo)), cut(tokens, lo), top_k)
+                 for lo in range(0, len(hidden), step)]
         return scoring.TokenLogprobs(*(torch.cat(p) for p in zip(*parts)))
 
 
@@ -97,6 +99,9 @@ def _sequences(page_ids: list, query_ids: list, separator_ids: list, start_ids: 
     return rows, [len(r) - len(query_ids) for r in rows]
 
 
+_FORWARD = threading.Lock()
+
+
 def page_scores(query: str, texts: list, model, tokenizer, head: ScoringHead, batch_size: int = 8, max_length: int = MAX_LENGTH) -> list:
     """Mean log probability of the query's tokens after each text, in nats."""
     encode = lambda t: list(tokenizer(t, add_special_tokens=False)["input_ids"])  # noqa: E731
@@ -111,11 +116,10 @@ def page_scores(query: str, texts: list, model, tokenizer, head: ScoringHead, ba
     rows, begins = _sequences([encode(t) for t in texts], query_ids, encode(SEPARATOR), start_ids, max_length)
     body, q = _body(model), len(query_ids)
     device = head.vocabulary.device
-    captured = []
-    hook = body.norm.register_forward_pre_hook(lambda module, args: captured.append(args[0]))
-    scores = []
-    try:
-        with torch.no_grad():
+    captured, scores = [], []
+    with _FORWARD, torch.no_grad():     # one thread at a time: the hook sees every forward of the model
+        hook = body.norm.register_forward_pre_hook(lambda module, args: captured.append(args[0]))
+        try:
             tokens = torch.tensor(query_ids, device=device)
             for lo in range(0, len(rows), batch_size):
                 part, at = rows[lo:lo + batch_size], begins[lo:lo + batch_size]
@@ -125,22 +129,28 @@ def page_scores(query: str, texts: list, model, tokenizer, head: ScoringHead, ba
                 for i, r in enumerate(part):
                     ids[i, :len(r)], mask[i, :len(r)] = torch.tensor(r), 1
                 captured.clear()
-                body(input_ids=ids.to(device), attention_mask=mask.to(device))
+                body(input_ids=ids.to(device), attention_mask=mask.to(device), use_cache=False)
                 hidden = captured[-1]
                 # the state at a position predicts the next token: from the one before the query to its last but one
                 where = (torch.tensor(at)[:, None] - 1 + torch.arange(q)[None]).to(device)
                 picked = hidden.gather(1, where[:, :, None].expand(-1, -1, hidden.shape[2])).reshape(-1, hidden.shape[2])
                 lp = head.token_logprobs(picked, tokens.repeat(len(part))).logprobs
                 scores.append(lp.reshape(len(part), q).mean(dim=1))
-    finally:
-        hook.remove()
+        finally:
+            hook.remove()
     return torch.cat(scores).tolist()
 
 
 _MODEL = {"key": None, "model": None, "tokenizer": None, "head": None}
+_LOADING = threading.Lock()
 
 
 def _model_for(model_name: str, device: str):
+    with _LOADING:
+        return _load(model_name, device)
+
+
+def _load(model_name: str, device: str):
     key = (model_name, device)
     if _MODEL["key"] == key:
         return _MODEL["model"], _MODEL["tokenizer"], _MODEL["head"]

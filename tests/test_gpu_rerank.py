@@ -97,6 +97,31 @@ def test_head_is_its_operators_and_is_cut_without_a_trace(loaded, monkeypatch):
         assert torch.equal(head.logits(hidden, res, torch.bfloat16), scoring.mx_matmul(rows, head.vocabulary, torch.bfloat16))
 
 
+def test_rows_taken_in_parts(loaded):
+    """More logits than are held at a time: the same results, with and without tokens and a residual."""
+    import torch
+
+    from medical_rag_amd import scoring
+    rerank, model, tok, head = loaded
+
+    class Few(rerank.ScoringHead):      # a vocabulary that counts as half a gigabyte of logits a row: four rows a part
+        class vocabulary_(scoring.MxRows):
+            __slots__ = ()
+
+            def __len__(self):
+                return 1 << 27
+
+    v = head.vocabulary
+    few = Few(head.norm_weight, head.eps, Few.vocabulary_(v.values, v.scales, v.d, v.format))
+    g = torch.Generator().manual_seed(1)
+    hidden, residual = (torch.randn(11, 96, generator=g).to(torch.bfloat16).cuda() for _ in range(2))
+    tokens = torch.randint(0, len(v), (11, 2), generator=g).cuda()
+    for tk in (None, tokens):
+        for res in (None, residual):
+            for a, b in zip(few.token_logprobs(hidden, tk, 4, res), head.token_logprobs(hidden, tk, 4, res)):
+                assert torch.equal(a, b)
+
+
 def test_rerank_pages_and_hits(loaded, decoder_dir):
     rerank, model, tok, head = loaded
     pages = [{"index": i, "text": t} for i, t in enumerate(PAGES)]
@@ -119,3 +144,16 @@ def test_caller_re_ranks_its_candidates(decoder_dir):
     idx, scores = got["pleural line"]
     assert len(idx) == 3 and set(idx.tolist()) <= set(plain["pleural line"][0].tolist()) and (np.diff(scores) <= 0).all()
     index.close()
+
+
+def test_two_threads_score_with_one_model(loaded):
+    """Each gets its own pages' scores, the ones it gets alone."""
+    from concurrent.futures import ThreadPoolExecutor
+    rerank, model, tok, head = loaded
+    lists = [PAGES[:3] * 8, PAGES[2:] * 8]
+    score = lambda pages: rerank.page_scores("pleural line", pages, model, tok, head, batch_size=3)  # noqa: E731
+    want = [score(p) for p in lists]
+    with ThreadPoolExecutor(2) as pool:
+        got = list(pool.map(score, lists * 3))
+    for i, g in enumerate(got):
+        assert g == want[i % 2]
