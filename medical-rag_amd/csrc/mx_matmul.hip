@@ -227,6 +227,13 @@ template <int FA, int MT, int NT, int KS, typename TO> hipError_t launch_rows(co
 
 constexpr int kTileThreads = 512, kTileN = 256;
 constexpr int kTileMaxGroups = 16384;       // offsets within a tile fit 32 bits
+// B's elements that all tiles of A are multiplied with before the next ones: they stay in the chip's 256 MB cache, and the
+// workgroups that run together write long pieces of few rows of out, which memory takes faster than short pieces of all rows
+// (measured, us, A's tiles running fastest / chunks of 24 MB / 40 MB / 96 MB / all of B at once: 511 x 100003 x 768 4 bits to
+// fp32 82 / 68 / 65 / 65 / 65, 500 x 1000000 x 768 4 bits to bf16 558 / 476 / 483 / 493 / 591, 2048 x 131072 x 4096 4 bits
+// 649 / 590 / 590 / 614 / 719, 8 bits 824 / 799 / 802 / 817 / 894, 1000 x 60000 x 4096 8 bits 198 / 200 / 201 / 205 / 202).  With
+// one tile of A neighbouring tiles on each XCD are faster (64 x 131072 x 4096 88 against 91).
+constexpr long long kChunkBytes = 40 << 20;
 
 // Scale bytes turned into the matrix instruction's order: for every K step and every 64 rows, 64 words
 // (row group x step, so a tile's words of one step lie together); word 16 g + r holds in its byte j the
@@ -272,7 +279,7 @@ struct TileArgs {
     const unsigned int *a_scales, *b_scales;    // turned: [groups][padded rows]
     long long m, n, m_padded, n_padded;
     int groups;
-    int m_tiles;
+    int m_tiles, n_tiles, chunk;
     void* out;
     long long ld;
     int whole, past;    // how results are stored: store4
@@ -334,10 +341,18 @@ __global__ __launch_bounds__(kTileThreads, 2 * PER_CU) void mx_matmul_tile_kerne
     const int lane = threadIdx.x & 63, r = lane & 15, g = lane >> 4;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int wm = wave / S::WN, wn = wave % S::WN;
-    // workgroups of one XCD take consecutive tiles, A's running fastest: they share rows of B in its L2
-    const int nwg = gridDim.x, xcd = blockIdx.x % 8, per = nwg / 8, rem = nwg % 8;
-    const int id = (xcd < rem ? xcd * (per + 1) : rem * (per + 1) + (xcd - rem) * per) + blockIdx.x / 8;
-    const long long m0 = (long long)(id % p.m_tiles) * S::M, n0 = (long long)(id / p.m_tiles) * kTileN;
+    int m_tile, n_tile;
+    if (p.m_tiles == 1) {       // workgroup b starts on XCD b % 8; each XCD takes neighbouring tiles
+        const int nwg = gridDim.x, xcd = blockIdx.x % 8, per = nwg / 8, rem = nwg % 8;
+        m_tile = 0;
+        n_tile = (xcd < rem ? xcd * (per + 1) : rem * (per + 1) + (xcd - rem) * per) + blockIdx.x / 8;
+    } else {                    // `chunk` tiles of B for all of A's tiles, then the next ones
+        const int before = blockIdx.x / (p.chunk * p.m_tiles) * p.chunk, in = blockIdx.x - before * p.m_tiles;
+        const int width = p.n_tiles - before < p.chunk ? p.n_tiles - before : p.chunk;
+        m_tile = in / width;
+        n_tile = before + in % width;
+    }
+    const long long m0 = (long long)m_tile * S::M, n0 = (long long)n_tile * kTileN;
 
     const unsigned int row_a = p.groups * S::kRowA, row_b = p.groups * 64;
     const unsigned char* a0 = p.a + m0 * row_a;
@@ -623,7 +638,9 @@ template <int FA, bool EXACT, int WM, int STAGES, int PER_CU, typename TO> hipEr
     const hipError_t e = hipFuncSetAttribute(fn, hipFuncAttributeMaxDynamicSharedMemorySize, lds);
     if (e != hipSuccess) return e;
     p.m_tiles = (int)((p.m + S::M - 1) / S::M);
-    const long long tiles = p.m_tiles * ((p.n + kTileN - 1) / kTileN);
+    p.n_tiles = (int)((p.n + kTileN - 1) / kTileN);
+    const long long tiles = (long long)p.m_tiles * p.n_tiles, chunk = kChunkBytes / ((long long)kTileN * 64 * p.groups) / 8 * 8;
+    p.chunk = (int)(chunk < 8 ? 8 : chunk < p.n_tiles ? chunk : p.n_tiles);
     if (tiles > 0x7fffff) return hipErrorInvalidValue;      // a launch counts its threads in 32 bits
     hipLaunchKernelGGL((mx_matmul_tile_kernel<FA, EXACT, WM, STAGES, PER_CU, TO>), dim3((unsigned int)tiles), dim3(kTileThreads), lds, stream, p);
     return hipGetLastError();
@@ -669,7 +686,7 @@ hipError_t launch_mx_matmul(const void* a_values, const void* a_scales, int a_fo
         const dim3 turn_grid((unsigned int)((up(m, 256) + up(n, 256)) / 64), (unsigned int)((groups + 31) / 32));
         hipLaunchKernelGGL(turn_scales_kernel, turn_grid, dim3(256), 0, stream, ta, tb, groups);
         if (const hipError_t e = hipGetLastError(); e != hipSuccess) return e;
-        const TileArgs p{a, b, as, bs, m, n, up(m, 256), up(n, 256), groups, 0, out, ld_out, whole, past};
+        const TileArgs p{a, b, as, bs, m, n, up(m, 256), up(n, 256), groups, 0, 0, 0, out, ld_out, whole, past};
         if (a_format == kMxFp4) return out_dtype == 0 ? tiles_4bit<float>(p, stream) : tiles_4bit<bf16_t>(p, stream);
         return out_dtype == 0 ? tiles_8bit<true, float>(p, stream) : tiles_8bit<false, bf16_t>(p, stream);
     }
