@@ -647,12 +647,15 @@ template <int FA, bool EXACT, int WM, int STAGES, int PER_CU, typename TO> hipEr
 }
 
 // Tiles of 64, 128 or 256 rows of A.  4-bit rows have room for two workgroups of the 128-row tile a CU, whose starts and
-// ends overlap, and take it where these weigh: short rows, or fewer tall tiles than CUs (measured, us, two workgroups /
-// tall: 511 x 100003 x 768 62 / 70, 1024 x 8192 x 4096 31 / 37, 2048 x 131072 x 4096 764 / 650).
+// ends overlap.  They take it where these weigh: with fewer tall tiles than CUs, or with short rows and a last round of tall
+// tiles (after few) that few CUs have one for (measured, us, two workgroups / tall: 1024 x 8192 x 4096 31 / 37; 511 rows, k = 768,
+// fp32: n = 40000, 1.2 rounds, 30 / 32, 100003, 3.05 rounds, 65 / 70, 128000, 3.9 rounds, 90 / 83, 200000, 6.1 rounds, 131 / 120;
+// k = 2048, 100003 110 / 97; 2048 x 131072 x 4096 764 / 650).
 template <typename TO> hipError_t tiles_4bit(const TileArgs& p, hipStream_t stream) {
     if (p.m <= 64) return launch_tiles<kMxFp4, false, 1, 3, 1, TO>(p, stream);
     const long long tall = (p.m + 255) / 256 * ((p.n + kTileN - 1) / kTileN);
-    if (p.m <= 128 || p.groups <= 8 || tall < 256) return launch_tiles<kMxFp4, false, 2, 3, 2, TO>(p, stream);
+    const bool few_last = tall < 4 * 256 && tall % 256 > 0 && tall % 256 <= 64;
+    if (p.m <= 128 || tall < 256 || (p.groups <= 8 && few_last)) return launch_tiles<kMxFp4, false, 2, 3, 2, TO>(p, stream);
     return launch_tiles<kMxFp4, false, 4, 3, 1, TO>(p, stream);
 }
 template <bool EXACT, typename TO> hipError_t tiles_8bit(const TileArgs& p, hipStream_t stream) {

@@ -272,6 +272,29 @@ def test_matmul_of_whole_numbers_is_exact(sc, fmt, out):
         assert torch.equal(got, product(va, vb).to(getattr(torch, out))), (m, n, d)
 
 
+@pytest.mark.parametrize("fmt", ["mxfp8", "mxfp4"])
+def test_matmul_through_several_chunks_of_b(sc, fmt):
+    """Rows so long that B's tiles are taken in chunks, the last one narrower; whole numbers, exact."""
+    import torch
+    g = torch.Generator(device="cuda").manual_seed(1)
+
+    def whole(n, d, fmt):
+        # a random element, its sign in the type's highest bit: 0, 1, 2, 3, 4, 6 in either type
+        few = torch.tensor([0, 2, 4, 5, 6, 7] if fmt == "mxfp4" else [0x00, 0x38, 0x40, 0x44, 0x48, 0x4C], dtype=torch.uint8, device="cuda")
+        codes = few[torch.randint(0, 6, (n, d), device="cuda", generator=g)]
+        codes |= torch.randint(0, 2, (n, d), device="cuda", generator=g, dtype=torch.uint8) << (3 if fmt == "mxfp4" else 7)
+        if fmt == "mxfp4":
+            codes = codes[:, ::2] | codes[:, 1::2] << 4
+        return sc.MxRows(codes.contiguous(), torch.full((n, d // 32), 127, dtype=torch.uint8, device="cuda"), d, fmt)
+
+    for m, n, d in ((300, 10500, 16384), (130, 24000, 8192)):
+        a, b = whole(m, d, fmt), whole(n, d, "mxfp4")
+        want = sc.mx_dequantize(a, torch.float32).double() @ sc.mx_dequantize(b, torch.float32).double().t()
+        assert float(want.abs().max()) > 0
+        for out in (torch.float32, torch.bfloat16):
+            assert torch.equal(sc.mx_matmul(a, b, out), want.to(out)), (m, n, d, out)
+
+
 def check_matmul(got, va, vb, fmt):
     """Sums of d products in fp32: d u sum |a b|.  (Products of an 8-bit element with a
     4-bit one have at most 6 bits, so they are exact.)  bf16 results of 8-bit rows may
