@@ -72,6 +72,23 @@ __device__ __forceinline__ u64 merge_reversed(u64 a, u64 reversed, int lane) {
     return exchanged<1>(c, lane);
 }
 
+// The 64 keys sorted, the best in lane 63 (zeros, which are no keys, first).
+template <int SIZE, int D> __device__ __forceinline__ u64 sorted_step(u64 c, int lane) {
+    const u64 o = ((u64)across<D>((unsigned int)(c >> 32), lane) << 32) | across<D>((unsigned int)c, lane);
+    const bool up = (lane & SIZE) == 0;                             // of this run of SIZE lanes
+    c = (((lane & D) == 0) == up) == (c < o) ? c : o;
+    if constexpr (D > 1) return sorted_step<SIZE, D / 2>(c, lane);
+    return c;
+}
+__device__ __forceinline__ u64 sorted_reversed(u64 c, int lane) {
+    c = sorted_step<2, 1>(c, lane);
+    c = sorted_step<4, 2>(c, lane);
+    c = sorted_step<8, 4>(c, lane);
+    c = sorted_step<16, 8>(c, lane);
+    c = sorted_step<32, 16>(c, lane);
+    return sorted_step<64, 32>(c, lane);
+}
+
 // A sorted list of 64 with one more key: everything below it moves one lane on.
 __device__ __forceinline__ u64 inserted(u64 key, u64 cand) {
     const unsigned int lo = (unsigned int)__builtin_amdgcn_update_dpp(-1, (int)(unsigned int)key, 0x138, 0xf, 0xf, false);          // the
@@ -180,15 +197,22 @@ __device__ __forceinline__ void write_row(const Outputs& o, long long row, const
 
 template <typename T> struct alignas(16) Piece { T v[16 / sizeof(T)]; };
 
+// How the list takes a round's candidates in.  One by one: about 25 instructions each.  With 12 alternatives and more, where
+// there are many, as in the first round, which fills the list, they are packed into one a lane through LDS, sorted (21
+// exchanges of 8 instructions) and merged (6); above 48 they are mostly more than the 64 that fit.  Measured (us, one by one /
+// sorted): 43 x 58112 bf16, 20 alternatives 20.5 / 18.1, 1 x 131072 fp32 14.6 / 12.8, 2048 x 131072 bf16 144 / 134, 64 of
+// 63 x 50257 33.7 / 37.4, 8 of 8 x 46760 12.0 / 13.1.
+constexpr int kTopNone = 0, kTopFew = 1, kTopMany = 2;
+
 // One workgroup a part of a row.  part_sums / part_keys: [row][split] and
 // [row][split][top_k]; with one split the row is finished here instead.
-template <typename T, bool TOP, int WAVES>
+template <typename T, int TOP, int WAVES>
 __global__ __launch_bounds__(64 * WAVES) void token_logprobs_kernel(Outputs o, int splits, long long part_len,
                                                                   Sums* __restrict__ part_sums, u64* __restrict__ part_keys) {
     constexpr int EPC = 16 / sizeof(T);                 // elements of a 16-byte load
     constexpr int U = 4;                                // loads a lane and round
     __shared__ Sums wave_sums[WAVES];
-    __shared__ u64 wave_keys[TOP ? WAVES * 64 : 1];
+    __shared__ u64 wave_keys[TOP != kTopNone ? WAVES * 64 : 1];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     const long long row = blockIdx.x / splits;
     const int split = (int)(blockIdx.x - row * splits);
@@ -237,15 +261,38 @@ __global__ __launch_bounds__(64 * WAVES) void token_logprobs_kernel(Outputs o, i
             for (int i = 1; i < U * EPC / 4; ++i) tops[q] = fmaxf(tops[q], x[q * (U * EPC / 4) + i]);
         }
         const float top = fmaxf(fmaxf(tops[0], tops[1]), fmaxf(tops[2], tops[3]));
-        if (__ballot(top > above)) {                    // wave-uniform, rare
+        const u64 better = __ballot(top > above);
+        if (better) {                                   // wave-uniform, rare
             float m = sums.m;
-            if constexpr (TOP) {
+            if constexpr (TOP != kTopNone) {
                 float least = above;                    // candidates reach it
                 if (kth == 0) {                         // a few of 64 parts' maxima say little less than of 256 parts'
                     const float one[1] = {top};
                     least = o.top_k <= 16 ? floor_of(one, o.top_k) : floor_of(tops, o.top_k);
                 }
                 least = fmaxf(least, -3.402823466e38f); // -inf is no candidate
+                u64* room = wave_keys + wave * 64;
+                int found = 0;
+                if (TOP == kTopMany && (kth == 0 || __popcll(better) >= 10)) {
+#pragma unroll
+                    for (int q = 0; q < 4; ++q) {
+                        if (!__ballot(tops[q] >= least)) continue;
+#pragma unroll
+                        for (int i = q * (U * EPC / 4); i < (q + 1) * (U * EPC / 4); ++i) {
+                            const u64 mask = __ballot(x[i] >= least);
+                            const int at = found + __builtin_amdgcn_mbcnt_hi((unsigned int)(mask >> 32), __builtin_amdgcn_mbcnt_lo((unsigned int)mask, 0));
+                            if (x[i] >= least && at < 64) room[at] = key_of(x[i], (unsigned int)(first + (i / EPC * 64 + lane) * EPC + i % EPC));
+                            found += __popcll(mask);
+                        }
+                    }
+                }
+                if (found > 0 && found <= 64) {
+                    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+                    const u64 c = lane < found ? room[lane] : 0;
+                    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+                    key = merge_reversed(key, sorted_reversed(c, lane), lane);
+                    kth = lane_key(key, o.top_k - 1);
+                } else
 #pragma unroll
                 for (int q = 0; q < 4; ++q) {
                     if (!__ballot(tops[q] >= least)) continue;
@@ -292,14 +339,14 @@ __global__ __launch_bounds__(64 * WAVES) void token_logprobs_kernel(Outputs o, i
         sums.s += __shfl_xor(sums.s, off, 64);
         sums.t += __shfl_xor(sums.t, off, 64);
     }
-    join_waves<WAVES, TOP>(sums, key, wave_sums, wave_keys, wave, lane);
+    join_waves<WAVES, TOP != kTopNone>(sums, key, wave_sums, wave_keys, wave, lane);
     if (wave != 0) return;
     if (splits == 1) {
         write_row<T>(o, row, sums, key, lane);
         return;
     }
     if (lane == 0) part_sums[row * splits + split] = sums;
-    if (TOP && lane < o.top_k) part_keys[(row * splits + split) * o.top_k + lane] = key;
+    if (TOP != kTopNone && lane < o.top_k) part_keys[(row * splits + split) * o.top_k + lane] = key;
 }
 
 // One workgroup a row: the parts' sums and lists joined.
@@ -345,7 +392,7 @@ Cut cut_for(long long n, long long v, int size) {
     return {4, (int)(want < most ? want : most)};
 }
 
-template <typename T, bool TOP> hipError_t launch_shaped(const Outputs& o, long long n, void* workspace, hipStream_t stream) {
+template <typename T, int TOP> hipError_t launch_shaped(const Outputs& o, long long n, void* workspace, hipStream_t stream) {
     const Cut c = cut_for(n, o.v, sizeof(T));
     const long long part_len = (o.v + c.splits - 1) / c.splits;
     Sums* sums = static_cast<Sums*>(workspace);
@@ -356,11 +403,13 @@ template <typename T, bool TOP> hipError_t launch_shaped(const Outputs& o, long 
     else if (c.waves == 8) hipLaunchKernelGGL((token_logprobs_kernel<T, TOP, 8>), grid, dim3(512), 0, stream, o, c.splits, part_len, sums, keys);
     else hipLaunchKernelGGL((token_logprobs_kernel<T, TOP, 4>), grid, dim3(256), 0, stream, o, c.splits, part_len, sums, keys);
     if (c.splits > 1)
-        hipLaunchKernelGGL((token_logprobs_join_kernel<T, TOP>), dim3((unsigned int)n), dim3(kJoinThreads), 0, stream, o, c.splits, sums, keys);
+        hipLaunchKernelGGL((token_logprobs_join_kernel<T, TOP != kTopNone>), dim3((unsigned int)n), dim3(kJoinThreads), 0, stream, o, c.splits, sums, keys);
     return hipGetLastError();
 }
 template <typename T> hipError_t launch_typed(const Outputs& o, long long n, void* workspace, hipStream_t stream) {
-    return o.top_k ? launch_shaped<T, true>(o, n, workspace, stream) : launch_shaped<T, false>(o, n, workspace, stream);
+    if (o.top_k == 0) return launch_shaped<T, kTopNone>(o, n, workspace, stream);
+    if (o.top_k < 12 || o.top_k > 48) return launch_shaped<T, kTopFew>(o, n, workspace, stream);
+    return launch_shaped<T, kTopMany>(o, n, workspace, stream);
 }
 
 }  // namespace

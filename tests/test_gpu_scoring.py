@@ -488,6 +488,21 @@ def test_ties_go_to_the_lower_id(sc):
     check_logprobs(sc, rising.flip(1).contiguous(), None, 64)
 
 
+@pytest.mark.parametrize("top_k", [11, 12, 13, 20, 48, 49])
+def test_alternatives_sorted_at_once_or_one_by_one(sc, top_k):
+    """Few and many candidates in the first and in later parts of a row, in orders that bring all or none of them late."""
+    import torch
+    for n, v in ((3, 20), (2, 300), (2, 5000), (5, 30000), (2, 140000)):
+        x = logits_of(n, v, "float32", seed=v)
+        check_logprobs(sc, x, None, top_k)
+        check_logprobs(sc, x.sort(dim=1).values.contiguous(), None, top_k)
+        check_logprobs(sc, x.sort(dim=1, descending=True).values.to(torch.bfloat16), None, top_k)
+        check_logprobs(sc, x.round().to(torch.float16), None, top_k)            # ties by the hundred
+        few = torch.full_like(x, -float("inf"))
+        few[:, ::max(1, v // 13)] = x[:, ::max(1, v // 13)]
+        check_logprobs(sc, few, None, top_k)
+
+
 def test_logits_strided_misaligned_and_far_apart(sc):
     import torch
     for dtype in DTYPES:
