@@ -101,7 +101,7 @@ __global__ __launch_bounds__(kThreads) void mx_dequantize_kernel(const unsigned 
             mx_decode4<FMT>(FMT == kMxFp4 ? q[u][0] & 0xffffu : q[u][0], s, f);
             mx_decode4<FMT>(FMT == kMxFp4 ? q[u][0] >> 16 : q[u][1], s, f + 4);
             if (VEC && col < d) store8<T>(o + col, f);
-            else store_some<T>(o + col, d - col, f);
+            else store_some<8>(o + col, d - col, f);
         } else {
 #pragma unroll
             for (int p = 0; p < 2; ++p) {
@@ -109,7 +109,7 @@ __global__ __launch_bounds__(kThreads) void mx_dequantize_kernel(const unsigned 
                 float f[8];
                 mx_decode4<FMT>(q[u][p], mx_scale((word[u] >> (8 * (2 * p + lane16 / 8))) & 255u), f);
                 if (VEC && col < d) *reinterpret_cast<f32x4*>(o + col) = f32x4{f[0], f[1], f[2], f[3]};
-                else store_some<T>(o + col, d - col < 4 ? d - col : 4, f);
+                else store_some<4>(o + col, d - col, f);
             }
         }
     }
@@ -149,7 +149,7 @@ __global__ __launch_bounds__(NT) void rms_norm_mx_kernel(const T* __restrict__ x
 #pragma unroll
             for (int i = 0; i < 8; ++i) h[c][i] = to_f32<T>(from_f32<T>(h[c][i] + r[i]));
             if (VEC && col < d) store8<T>(residual_out + row * d + col, h[c]);
-            else store_some<T>(residual_out + row * d + col, d - col, h[c]);
+            else store_some<8>(residual_out + row * d + col, d - col, h[c]);
         }
     }
 #pragma unroll

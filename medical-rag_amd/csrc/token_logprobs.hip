@@ -198,10 +198,11 @@ __device__ __forceinline__ void write_row(const Outputs& o, long long row, const
 template <typename T> struct alignas(16) Piece { T v[16 / sizeof(T)]; };
 
 // How the list takes a round's candidates in.  One by one: about 25 instructions each.  With 12 alternatives and more, where
-// there are many, as in the first round, which fills the list, they are packed into one a lane through LDS, sorted (21
-// exchanges of 8 instructions) and merged (6); above 48 they are mostly more than the 64 that fit.  Measured (us, one by one /
-// sorted): 43 x 58112 bf16, 20 alternatives 20.5 / 18.1, 1 x 131072 fp32 14.6 / 12.8, 2048 x 131072 bf16 144 / 134, 64 of
-// 63 x 50257 33.7 / 37.4, 8 of 8 x 46760 12.0 / 13.1.
+// there are many, as in the first round, which fills the list, they are packed through LDS, 64 at a time sorted (21 exchanges
+// of 8 instructions) and merged (6); more than kRoom go one by one.  Measured (us, one by one / sorted): 43 x 58112 bf16, 20
+// alternatives 20.5 / 18.1, 1 x 131072 fp32 14.6 / 12.8, 2048 x 131072 bf16 144 / 134, 64 of 63 x 50257 fp16 33.7 / 18.4, 8 of
+// 8 x 46760 12.0 / 13.1.
+constexpr int kRoom = 128;
 constexpr int kTopNone = 0, kTopFew = 1, kTopMany = 2;
 
 // One workgroup a part of a row.  part_sums / part_keys: [row][split] and
@@ -213,6 +214,7 @@ __global__ __launch_bounds__(64 * WAVES) void token_logprobs_kernel(Outputs o, i
     constexpr int U = 4;                                // loads a lane and round
     __shared__ Sums wave_sums[WAVES];
     __shared__ u64 wave_keys[TOP != kTopNone ? WAVES * 64 : 1];
+    __shared__ u64 rooms[TOP == kTopMany ? WAVES * kRoom : 1];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     const long long row = blockIdx.x / splits;
     const int split = (int)(blockIdx.x - row * splits);
@@ -271,7 +273,7 @@ __global__ __launch_bounds__(64 * WAVES) void token_logprobs_kernel(Outputs o, i
                     least = o.top_k <= 16 ? floor_of(one, o.top_k) : floor_of(tops, o.top_k);
                 }
                 least = fmaxf(least, -3.402823466e38f); // -inf is no candidate
-                u64* room = wave_keys + wave * 64;
+                u64* room = rooms + (TOP == kTopMany ? wave * kRoom : 0);
                 int found = 0;
                 if (TOP == kTopMany && (kth == 0 || __popcll(better) >= 10)) {
 #pragma unroll
@@ -281,16 +283,18 @@ __global__ __launch_bounds__(64 * WAVES) void token_logprobs_kernel(Outputs o, i
                         for (int i = q * (U * EPC / 4); i < (q + 1) * (U * EPC / 4); ++i) {
                             const u64 mask = __ballot(x[i] >= least);
                             const int at = found + __builtin_amdgcn_mbcnt_hi((unsigned int)(mask >> 32), __builtin_amdgcn_mbcnt_lo((unsigned int)mask, 0));
-                            if (x[i] >= least && at < 64) room[at] = key_of(x[i], (unsigned int)(first + (i / EPC * 64 + lane) * EPC + i % EPC));
+                            if (x[i] >= least && at < kRoom) room[at] = key_of(x[i], (unsigned int)(first + (i / EPC * 64 + lane) * EPC + i % EPC));
                             found += __popcll(mask);
                         }
                     }
                 }
-                if (found > 0 && found <= 64) {
+                if (found > 0 && found <= kRoom) {
                     __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-                    const u64 c = lane < found ? room[lane] : 0;
+                    for (int b = 0; b < found; b += 64) {
+                        const u64 c = b + lane < found ? room[b + lane] : 0;
+                        key = merge_reversed(key, sorted_reversed(c, lane), lane);
+                    }
                     __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-                    key = merge_reversed(key, sorted_reversed(c, lane), lane);
                     kth = lane_key(key, o.top_k - 1);
                 } else
 #pragma unroll
@@ -408,7 +412,7 @@ template <typename T, int TOP> hipError_t launch_shaped(const Outputs& o, long l
 }
 template <typename T> hipError_t launch_typed(const Outputs& o, long long n, void* workspace, hipStream_t stream) {
     if (o.top_k == 0) return launch_shaped<T, kTopNone>(o, n, workspace, stream);
-    if (o.top_k < 12 || o.top_k > 48) return launch_shaped<T, kTopFew>(o, n, workspace, stream);
+    if (o.top_k < 12) return launch_shaped<T, kTopFew>(o, n, workspace, stream);
     return launch_shaped<T, kTopMany>(o, n, workspace, stream);
 }
 
