@@ -4,11 +4,17 @@
     rocprofv3 --kernel-trace --output-format csv -d DIR -- python3 profiles/scoring_head.py
     python3 profiles/scoring_head.py summary DIR/.../*_kernel_trace.csv > profiles/scoring_head_kernel_stats.csv
 
+    rocprofv3 --pmc SQ_BUSY_CU_CYCLES ... --kernel-trace --output-format csv -d DIR -- python3 profiles/scoring_head.py
+    python3 profiles/scoring_head.py counters DIR/.../*_counter_collection.csv > profiles/scoring_head_pmc.json
+
 The first runs every case REPEATS times on inputs that lie in memory; the second
 writes, per case and kernel, the number of launches a call, the median time and what
-the case's bytes and operations make of it."""
+the case's bytes and operations make of it; the third the means of the counters that
+were collected, per kernel."""
 import csv
+import json
 import os
+import re
 import sys
 
 sys.path.insert(0, os.path.dirname(os.path.dirname(os.path.abspath(__file__))))
@@ -94,10 +100,20 @@ def summary(path):
             mine = [c for c in calls if c[0] == kernel]
             us = sorted(c[1] for c in mine)[len(mine) // 2]
             main = "join" not in kernel and "turn" not in kernel
-            short = kernel.split("(anonymous namespace)::")[-1].split("(")[0]
+            short = re.search(r"(mx|rms_norm|turn_scales|token_logprobs)\w*_kernel", kernel).group(0)
             out.writerow([name, short, f"{len(mine) / REPEATS:g}", f"{mine[0][2]}", f"{us:.2f}", f"{size / us / 1e3:.0f}" if main else "",
                           f"{flops / us / 1e6:.0f}" if main and flops else ""])
 
 
+def counters(path):
+    out = {}
+    for r in csv.DictReader(open(path)):
+        kernel = re.search(r"(mx|rms_norm|turn_scales|token_logprobs)\w*_kernel(<[^>]*>|I\w*E(?=Ev))?", r["Kernel_Name"])
+        if kernel:
+            of = out.setdefault(f"{kernel.group(0)}, {r['Grid_Size']} threads", {})
+            of.setdefault(r["Counter_Name"], {})[r["Dispatch_Id"]] = float(r["Counter_Value"])
+    print(json.dumps({k: {c: round(sum(d.values()) / len(d)) for c, d in v.items()} for k, v in out.items()}, indent=1))
+
+
 if __name__ == "__main__":
-    summary(sys.argv[2]) if sys.argv[1:2] == ["summary"] else run()
+    {"summary": summary, "counters": counters}[sys.argv[1]](sys.argv[2]) if len(sys.argv) > 1 else run()
