@@ -16,7 +16,11 @@
 //
 // Two kernels.  Few rows of A, or few of both, are bound by the one pass over B or by
 // how many waves there are: every wave takes its rows of B straight from memory into
-// its operand registers.  Larger products take tiles staged in LDS.
+// its operand registers (1 x 131072 x 4096, 8 bits: 52 us, 5.5 TB/s).  Larger products
+// take tiles staged in LDS.  2048 x 131072 x 4096: both 4 bits 580 us, 3.8 PFLOP/s, 8
+// bits to bfloat16 794 us, 2.8 PFLOP/s with the matrix cores busy 71 % of the cycles at
+// the 1.85 GHz that the chip holds under it, 8 bits to fp32 1.68 ms, 1.3 PFLOP/s, bound by the
+// conversions beside the bfloat16 instruction.
 #include "mx_format.h"
 
 namespace mtr {
@@ -239,7 +243,8 @@ constexpr long long kChunkBytes = 40 << 20;
 // (row group x step, so a tile's words of one step lie together); word 16 g + r holds in its byte j the
 // scale of block g of row 16 j + r, so that a lane finds in ONE word its scales for four operands, which
 // the instruction picks by byte.  Read where they are, each row's four bytes would cost a request of their
-// own, as many as the elements' do.
+// own, as many as the elements' do.  (4 bytes of every 64 or 128 of elements, read and written once: 5 us for 511 x
+// 100003 x 768, 10 us for 2048 x 131072 x 4096.)
 struct Turn {
     const unsigned int* src;    // [rows][groups]
     long long rows, padded_rows;
@@ -434,7 +439,7 @@ __global__ __launch_bounds__(kTileThreads, 2 * PER_CU) void mx_matmul_tile_kerne
         constexpr int H = S::NT / 2, kReadsA = FA == kMxFp4 ? 1 : 2;
         // Loads of a step that go out in a second half; the rest goes out in the next first half.  Half of them where the
         // multiplications of half a step are over before all loads are out: 4-bit rows in the tall tile (2048 x 131072 x
-        // 4096 672 -> 650 us; short products, which the tall tile is not for, would lose by the later start).
+        // 4096 607 -> 599 us; short products, which the tall tile is not for, would lose by the later start).
         constexpr int kEarly = FA == kMxFp4 && WM == 4 ? (S::kLoads + 1) / 2 : S::kLoads;
 #pragma unroll
         for (int s = 0; s < STAGES; ++s)
@@ -609,14 +614,14 @@ __global__ __launch_bounds__(kTileThreads, 2 * PER_CU) void mx_matmul_tile_kerne
 
 
 // Tiles fill the chip from about 48 of them on; below, and for rows too long for their 32-bit offsets, every wave
-// on its own is faster (measured, k = 4096, 8 bits to fp32, microseconds, tiles / waves: 32 x 131072 96 / 109,
-// 16 x 131072 91 / 76, 256 x 16384 99 / 88, 512 x 16384 101 / 172, 512 x 4032 97 / 46, 1024 x 4032 100 / 88).
+// on its own is faster (measured, k = 4096, 8 bits to fp32, microseconds, tiles / waves: 32 x 131072 100 / 110,
+// 16 x 131072 87 / 78, 256 x 16384 99 / 88, 512 x 16384 99 / 173, 512 x 4032 97 / 47, 1024 x 4032 98 / 88).
 bool takes_tiles(long long m, long long n, int groups) { return m * n > 3000000 && groups <= kTileMaxGroups; }
 
 template <int FA, int MT, typename TO> hipError_t rows_split(const MatmulArgs& p, hipStream_t stream) {
     // 16 rows of B a wave while that gives no CU a second workgroup, else 32; K split over four waves until there are
-    // waves enough without (measured, k = 4096, 8 bits, microseconds: 64 x 4032 12.5 with 16 rows / 14.2 with 32,
-    // 128 x 4032 22 / 15; 256 x 4032 29.6 split / 44.8 not, 512 x 4032 55.5 / 46.3, 16 x 131072 81 / 76).
+    // waves enough without (measured, k = 4096, 8 bits, microseconds: 64 x 4032 11.7 with 16 rows / 14.1 with 32,
+    // 128 x 4032 22 / 15; 256 x 4032 28 split / 45 not, 512 x 4032 53 / 45, 16 x 131072 83 / 76).
     const long long m_tiles = (p.m + 16 * MT - 1) / (16 * MT), narrow = m_tiles * ((p.n + 15) / 16);
     if (narrow <= 256) return launch_rows<FA, MT, 1, 4, TO>(p, stream);
     if (narrow / 2 < (MT == 1 ? 4000 : 1000)) return launch_rows<FA, MT, 2, 4, TO>(p, stream);
@@ -648,9 +653,9 @@ template <int FA, bool EXACT, int WM, int STAGES, int PER_CU, typename TO> hipEr
 
 // Tiles of 64, 128 or 256 rows of A.  4-bit rows have room for two workgroups of the 128-row tile a CU, whose starts and
 // ends overlap.  They take it where these weigh: with fewer tall tiles than CUs, or with short rows and a last round of tall
-// tiles (after few) that few CUs have one for (measured, us, two workgroups / tall: 1024 x 8192 x 4096 31 / 37; 511 rows, k = 768,
+// tiles (after few) that few CUs have one for (measured, us, two workgroups / tall: 1024 x 8192 x 4096 30 / 34; 511 rows, k = 768,
 // fp32: n = 40000, 1.2 rounds, 30 / 32, 100003, 3.05 rounds, 65 / 70, 128000, 3.9 rounds, 90 / 83, 200000, 6.1 rounds, 131 / 120;
-// k = 2048, 100003 110 / 97; 2048 x 131072 x 4096 764 / 650).
+// k = 2048, 100003 110 / 97; 2048 x 131072 x 4096 707 / 597).
 template <typename TO> hipError_t tiles_4bit(const TileArgs& p, hipStream_t stream) {
     if (p.m <= 64) return launch_tiles<kMxFp4, false, 1, 3, 1, TO>(p, stream);
     const long long tall = (p.m + 255) / 256 * ((p.n + kTileN - 1) / kTileN);

@@ -20,6 +20,10 @@
 // preserving form above the complement of the id: larger logits first, then lower
 // ids.  Most of the row costs one comparison of a lane's 16 or 32 logits' maximum with the
 // k-th best so far.
+//
+// Bound by the one pass over the logits where there are many (2048 x 131072 bf16, one alternative:
+// 86 us, 6.2 TB/s), else by the latency of the selection and of the join (1 x 131072 fp32, 20
+// alternatives: 6.9 us and 6.0 us to join 32 parts).
 #include "mx_format.h"
 
 namespace mtr {
@@ -379,11 +383,12 @@ __global__ __launch_bounds__(kJoinThreads) void token_logprobs_join_kernel(Outpu
     if (wave == 0) write_row<T>(o, row, sums, key, lane);
 }
 
-// How rows are cut (measured, microseconds).  Waves of a workgroup, one a row: 4 for short rows (4096 x 8000 bf16 28, with
-// 8 44, with 16 76) and where there are rows for every CU several times over (2048 x 100003 bf16 84 / 91 / 101), 8 there
-// from about 200 KB a row on (2048 x 131072 bf16 116 / 104 / 114), 16 for fewer long rows (256 x 131072 fp32 41 / 28 / 26).
+// How rows are cut (measured, microseconds).  Waves of a workgroup, one a row: 4 for short rows (4096 x 8000 bf16 22, with
+// 8 37, with 16 95) and where there are rows for every CU several times over, 8 there from
+// about 200 KB a row on (2048 x 100003 bf16 87 / 84 / 123, 2048 x 131072 101 / 90 / 122), 16 for fewer long rows (256 x 131072
+// fp32 38 / 27 / 26).
 // Parts of a row, of four waves and at least 4096 logits, only for less than 128 rows that are longer still, as a second
-// launch then joins them (1 x 131072 fp32, 20 alternatives: 15 in 32 parts, 36 whole; 63 x 50257 fp16: 16 in 12 parts, 15 whole).
+// launch then joins them (1 x 131072 fp32, 20 alternatives: 12.5 in 32 parts, 28 whole; 63 x 50257 fp16: 15 in 12 parts, 13 whole).
 struct Cut {
     int waves, splits;
 };
