@@ -116,6 +116,26 @@ def test_dequantize_rounds_once(sc, dtype, fmt):
         assert got.dtype == want.dtype and torch.equal(got.cpu(), want)
 
 
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("fmt", ["mxfp4", "mxfp8"])
+def test_dequantize_at_every_width_and_address(sc, dtype, fmt):
+    """Into rows that start anywhere, with what lies between and behind them left alone; blocks of very different scales."""
+    import torch
+    dt = getattr(torch, dtype)
+    for d in list(range(1, 18)) + [31, 33, 63, 65, 95, 97, 120, 121, 125, 126, 127, 128, 129, 135, 136, 250, 255, 257]:
+        x = rows(5, d, "float32", seed=d) * torch.exp2(torch.randint(-6, 6, (1, d), generator=torch.Generator().manual_seed(d)).float()).cuda()
+        q = sc.mx_quantize(x, fmt)
+        want = sc.mx_dequantize(q, torch.float32).to(dt)
+        for start in range(9):
+            for gap in (0, 1, 8):
+                flat = torch.full((5 * (d + gap) + 32,), 7.0, dtype=dt, device="cuda")
+                out = flat[start:start + 5 * (d + gap)].view(5, d + gap)[:, :d]
+                sc.mx_dequantize(q, out=out)
+                assert torch.equal(out, want), (d, start, gap)
+                out.fill_(7.0)
+                assert bool((flat == 7.0).all()), (d, start, gap)
+
+
 def test_every_code_and_scale_reads_back(sc):
     """All 256 bytes under all 256 scale bytes, e4m3's own NaNs included."""
     import torch
