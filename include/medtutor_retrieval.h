@@ -302,7 +302,8 @@ int mtr_rms_norm_mx(const void* dev_x, const void* dev_residual, const void* dev
                     int32_t format, void* dev_residual_out, void* dev_values, void* dev_scales,
                     int32_t device_id, void* stream);
 /* out[m][n] = A (m rows of d, either format) times the transpose of B (n rows of d,
- * MTR_MX_FP4), MTR_F32 or MTR_BF16; m and n up to MTR_MX_MATMUL_MAX_ROWS.
+ * MTR_MX_FP4), MTR_F32 or MTR_BF16, summed in 32 bits and rounded once; m and n up
+ * to MTR_MX_MATMUL_MAX_ROWS.
  * Workspace: mtr_mx_matmul_workspace bytes on 4 bytes, the caller's, not shared by
  * calls that may overlap. */
 #define MTR_MX_MATMUL_MAX_ROWS 536870912

@@ -1,26 +1,23 @@
 // Product of microscaled rows: out[m][n] = A [m][k] times the transpose of B [n][k], A in
 // 8 or 4 bits, B (a vocabulary matrix, an index) in 4.
 //
-// Two ways to multiply on the matrix cores (measured on normal data with k = 4096,
-// against 64 bits):
+// Two ways to multiply on the matrix cores:
 //   v_mfma_scale_f32_16x16x128_f8f6f4 takes both operands and their scales as stored.
 //     With 4-bit operands on both sides its sums are exact to 32 bits; with an 8-bit
-//     operand it keeps about 16 bits of a product relative to the largest of the 128 it
-//     sums (2-norm error 6e-6 to 3e-5).
+//     operand it keeps about 16 bits of the largest of the 128 products it sums, so that
+//     a few large elements in a row take away the rest of its sum (rows whose columns'
+//     magnitudes spread by e^3: off by 2^-13 of the sum of the products' magnitudes).
 //   v_mfma_f32_16x16x32_bf16 on both operands times their scales, which bfloat16 holds
 //     exactly: sums as exact as 32 bits allow, at half the rate and with the conversions.
-// 4-bit rows take the first.  8-bit rows take the second where few rows make the
-// product wait for memory anyway or the results are kept in 32 bits, and the first
-// where they are rounded to bfloat16, whose half step of 4e-3 is a hundred times the
-// difference.
+// 4-bit rows take the first, 8-bit rows the second (2048 x 131072 x 4096 to bfloat16 0.79 ms
+// with the first): sums are held in 32 bits whatever the sizes and the result's type.
 //
 // Two kernels.  Few rows of A, or few of both, are bound by the one pass over B or by
 // how many waves there are: every wave takes its rows of B straight from memory into
 // its operand registers (1 x 131072 x 4096, 8 bits: 52 us, 5.5 TB/s).  Larger products
 // take tiles staged in LDS.  2048 x 131072 x 4096: both 4 bits 580 us, 3.8 PFLOP/s, 8
-// bits to bfloat16 794 us, 2.8 PFLOP/s with the matrix cores busy 71 % of the cycles at
-// the 1.85 GHz that the chip holds under it, 8 bits to fp32 1.68 ms, 1.3 PFLOP/s, bound by the
-// conversions beside the bfloat16 instruction.
+// bits to bfloat16 1.60 ms, 1.4 PFLOP/s, bound by the conversions beside the bfloat16
+// instruction.
 #include "mx_format.h"
 
 namespace mtr {
@@ -235,8 +232,7 @@ constexpr int kTileMaxGroups = 16384;       // offsets within a tile fit 32 bits
 // workgroups that run together write long pieces of few rows of out, which memory takes faster than short pieces of all rows
 // (measured, us, A's tiles running fastest / chunks of 24 MB / 40 MB / 96 MB / all of B at once: 511 x 100003 x 768 4 bits to
 // fp32 82 / 68 / 65 / 65 / 65, 500 x 1000000 x 768 4 bits to bf16 558 / 476 / 483 / 493 / 591, 2048 x 131072 x 4096 4 bits
-// 649 / 590 / 590 / 614 / 719, 8 bits 824 / 799 / 802 / 817 / 894, 1000 x 60000 x 4096 8 bits 198 / 200 / 201 / 205 / 202).  With
-// one tile of A neighbouring tiles on each XCD are faster (64 x 131072 x 4096 88 against 91).
+// 649 / 590 / 590 / 614 / 719).  With one tile of A neighbouring tiles on each XCD are faster (64 x 131072 x 4096 88 against 91).
 constexpr long long kChunkBytes = 40 << 20;
 
 // Scale bytes turned into the matrix instruction's order: for every K step and every 64 rows, 64 words
@@ -305,11 +301,9 @@ __device__ __forceinline__ void barrier_keeping_loads() {
     asm volatile("" ::: "memory");
 }
 
-// The scaled instruction with the operands' scales in bytes ib and ia of their words.
-template <int FA> __device__ __forceinline__ f32x4 scaled_mfma(const i32x8& fb, const i32x8& fa, const f32x4& c, unsigned int xb, int ib,
-                                                               unsigned int xa, int ia) {
-    constexpr int kB = FA == kMxFp4 ? 4 : 0;
-#define MTR_BYTES(B, A) if (ib == B && ia == A) return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(fb, fa, c, 4, kB, B, (int)xb, A, (int)xa);
+// The scaled instruction on 4-bit operands with their scales in bytes ib and ia of their words.
+__device__ __forceinline__ f32x4 scaled_mfma(const i32x8& fb, const i32x8& fa, const f32x4& c, unsigned int xb, int ib, unsigned int xa, int ia) {
+#define MTR_BYTES(B, A) if (ib == B && ia == A) return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(fb, fa, c, 4, 4, B, (int)xb, A, (int)xa);
     MTR_BYTES(0, 0) MTR_BYTES(0, 1) MTR_BYTES(0, 2) MTR_BYTES(0, 3) MTR_BYTES(1, 0) MTR_BYTES(1, 1) MTR_BYTES(1, 2) MTR_BYTES(1, 3)
     MTR_BYTES(2, 0) MTR_BYTES(2, 1) MTR_BYTES(2, 2) MTR_BYTES(2, 3) MTR_BYTES(3, 0) MTR_BYTES(3, 1) MTR_BYTES(3, 2) MTR_BYTES(3, 3)
 #undef MTR_BYTES
@@ -326,22 +320,22 @@ template <int FA> __device__ __forceinline__ f32x4 scaled_mfma(const i32x8& fb, 
 // in four parts of 16 lanes, {0-3, 12-15, 20-27}, {4-11, 16-19, 28-31} and the same
 // 32 lanes on (measured), from 64 banks; with the row's low three bits (rows of 128
 // bytes) or its bits 1 and 2 (64 bytes) in the chunk number no part meets a bank twice.
-template <int FA, bool EXACT, int WM, int STAGES> struct Tile {
+template <int FA, int WM, int STAGES> struct Tile {
     static constexpr int M = 64 * WM, WN = 8 / WM, NT = kTileN / WN / 16, MT = 4;
     static constexpr int kRowA = FA == kMxFp4 ? 64 : 128;       // bytes of a row of A a step
     static constexpr int kBytesA = M * kRowA, kBytesB = kTileN * 64;
     static constexpr int kStage = kBytesA + kBytesB + 2048;     // 512 scale words: A's M, B's 256, the rest unused
     static constexpr int kLoadsA = kBytesA < 8192 ? 1 : kBytesA / 8192, kLoadsB = kBytesB / 8192, kLoads = kLoadsA + kLoadsB + 1;
     // Which 16-byte chunk of an 8-bit row lies (before the swizzle) in place q: lanes read places g and 4 + g, which
-    // hold elements 16 g .. and 64 + 16 g .. for the scaled instruction, 32 g .. and 32 g + 16 .. for the other.
-    static __device__ __forceinline__ int chunk8(int q) { return EXACT ? (q & 3) * 2 + q / 4 : q; }
+    // hold elements 32 g .. and 32 g + 16 ...
+    static __device__ __forceinline__ int chunk8(int q) { return (q & 3) * 2 + q / 4; }
     // The wave's i-th piece (1 KiB) of A; with fewer pieces than waves several load the same one.
     static __device__ __forceinline__ int piece_a(int wave, int i) { return (wave * kLoadsA + i) % (kBytesA / 1024); }
 };
 
-template <int FA, bool EXACT, int WM, int STAGES, int PER_CU, typename TO>
+template <int FA, int WM, int STAGES, int PER_CU, typename TO>
 __global__ __launch_bounds__(kTileThreads, 2 * PER_CU) void mx_matmul_tile_kernel(TileArgs p) {
-    using S = Tile<FA, EXACT, WM, STAGES>;
+    using S = Tile<FA, WM, STAGES>;
     extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
     const int lane = threadIdx.x & 63, r = lane & 15, g = lane >> 4;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -419,28 +413,22 @@ __global__ __launch_bounds__(kTileThreads, 2 * PER_CU) void mx_matmul_tile_kerne
 #pragma unroll
         for (int i = 0; i < kWords; ++i) xb[i] = words[S::M + (wn * S::NT / 4 + i) * 64 + lane] >> (S::NT < 4 ? wn % 2 * 16 : 0);
     };
-    if constexpr (!EXACT) {
+    if constexpr (FA == kMxFp4) {
         i32x8 fa[S::MT];
         i32x4 fb[S::NT];
         const auto read_a = [&](const unsigned char* st, int j) {
             const unsigned char* row = st + (wm * 64 + j * 16 + r) * S::kRowA;
-            if constexpr (FA == kMxFp4) {
-                const i32x4 v = *reinterpret_cast<const i32x4*>(row + ((g ^ ((r >> 1) & 3)) << 4));
-                fa[j] = __builtin_shufflevector(v, v, 0, 1, 2, 3, -1, -1, -1, -1);
-            } else {        // the instruction takes elements 16 g .. and 64 + 16 g .. of an 8-bit row
-                const i32x4 v = *reinterpret_cast<const i32x4*>(row + ((g ^ (r & 7)) << 4));
-                const i32x4 w = *reinterpret_cast<const i32x4*>(row + (((4 + g) ^ (r & 7)) << 4));
-                fa[j] = __builtin_shufflevector(v, w, 0, 1, 2, 3, 4, 5, 6, 7);
-            }
+            const i32x4 v = *reinterpret_cast<const i32x4*>(row + ((g ^ ((r >> 1) & 3)) << 4));
+            fa[j] = __builtin_shufflevector(v, v, 0, 1, 2, 3, -1, -1, -1, -1);
         };
         const auto read_b = [&](const unsigned char* st, int i) {
             fb[i] = *reinterpret_cast<const i32x4*>(st + S::kBytesA + ((wn * S::NT + i) * 16 + r) * 64 + ((g ^ ((r >> 1) & 3)) << 4));
         };
-        constexpr int H = S::NT / 2, kReadsA = FA == kMxFp4 ? 1 : 2;
+        constexpr int H = S::NT / 2;
         // Loads of a step that go out in a second half; the rest goes out in the next first half.  Half of them where the
-        // multiplications of half a step are over before all loads are out: 4-bit rows in the tall tile (2048 x 131072 x
+        // multiplications of half a step are over before all loads are out: in the tall tile (2048 x 131072 x
         // 4096 607 -> 599 us; short products, which the tall tile is not for, would lose by the later start).
-        constexpr int kEarly = FA == kMxFp4 && WM == 4 ? (S::kLoads + 1) / 2 : S::kLoads;
+        constexpr int kEarly = WM == 4 ? (S::kLoads + 1) / 2 : S::kLoads;
 #pragma unroll
         for (int s = 0; s < STAGES; ++s)
 #pragma unroll
@@ -468,7 +456,7 @@ __global__ __launch_bounds__(kTileThreads, 2 * PER_CU) void mx_matmul_tile_kerne
             for (int i = 0; i < H; ++i)
 #pragma unroll
                 for (int j = 0; j < S::MT; ++j)
-                    acc[i][j] = scaled_mfma<FA>(__builtin_shufflevector(fb[i], fb[i], 0, 1, 2, 3, -1, -1, -1, -1), fa[j], acc[i][j], xb[i / 4],
+                    acc[i][j] = scaled_mfma(__builtin_shufflevector(fb[i], fb[i], 0, 1, 2, 3, -1, -1, -1, -1), fa[j], acc[i][j], xb[i / 4],
                                                 i % 4, xa, j);
 #pragma unroll
             for (int i = 0; i < H; ++i) {
@@ -493,7 +481,7 @@ __global__ __launch_bounds__(kTileThreads, 2 * PER_CU) void mx_matmul_tile_kerne
             for (int j = 0; j < S::MT; ++j) {
 #pragma unroll
                 for (int i = H; i < S::NT; ++i)
-                    acc[i][j] = scaled_mfma<FA>(__builtin_shufflevector(fb[i], fb[i], 0, 1, 2, 3, -1, -1, -1, -1), fa[j], acc[i][j], xb[i / 4],
+                    acc[i][j] = scaled_mfma(__builtin_shufflevector(fb[i], fb[i], 0, 1, 2, 3, -1, -1, -1, -1), fa[j], acc[i][j], xb[i / 4],
                                                 i % 4, xa, j);
                 read_a(st1, j);
                 if (j < H) read_b(st1, j);
@@ -504,13 +492,13 @@ __global__ __launch_bounds__(kTileThreads, 2 * PER_CU) void mx_matmul_tile_kerne
 #pragma unroll
             for (int j = 0; j < H; ++j) {
                 __builtin_amdgcn_sched_group_barrier(0x008, S::NT - H, 0);
-                __builtin_amdgcn_sched_group_barrier(0x100, kReadsA + 1, 0);
+                __builtin_amdgcn_sched_group_barrier(0x100, 2, 0);
                 __builtin_amdgcn_sched_group_barrier(0x020, (kEarly + S::MT - 1) / S::MT, 0);
             }
 #pragma unroll
             for (int j = H; j < S::MT; ++j) {
                 __builtin_amdgcn_sched_group_barrier(0x008, S::NT - H, 0);
-                __builtin_amdgcn_sched_group_barrier(0x100, kReadsA, 0);
+                __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
                 __builtin_amdgcn_sched_group_barrier(0x020, (kEarly + S::MT - 1) / S::MT, 0);
             }
             xa = ya;
@@ -635,10 +623,10 @@ template <int FA, typename TO> hipError_t rows_shaped(const MatmulArgs& p, hipSt
 
 long long up(long long x, long long to) { return (x + to - 1) / to * to; }
 
-template <int FA, bool EXACT, int WM, int STAGES, int PER_CU, typename TO> hipError_t launch_tiles(TileArgs p, hipStream_t stream) {
-    using S = Tile<FA, EXACT, WM, STAGES>;
+template <int FA, int WM, int STAGES, int PER_CU, typename TO> hipError_t launch_tiles(TileArgs p, hipStream_t stream) {
+    using S = Tile<FA, WM, STAGES>;
     constexpr int lds = STAGES * S::kStage;
-    const void* fn = reinterpret_cast<const void*>(&mx_matmul_tile_kernel<FA, EXACT, WM, STAGES, PER_CU, TO>);
+    const void* fn = reinterpret_cast<const void*>(&mx_matmul_tile_kernel<FA, WM, STAGES, PER_CU, TO>);
     static_assert(PER_CU * lds <= 160 * 1024 && 8 * 16 * (S::NT * 16 + 4) * 4 <= lds, "LDS");
     const hipError_t e = hipFuncSetAttribute(fn, hipFuncAttributeMaxDynamicSharedMemorySize, lds);
     if (e != hipSuccess) return e;
@@ -647,7 +635,7 @@ template <int FA, bool EXACT, int WM, int STAGES, int PER_CU, typename TO> hipEr
     const long long tiles = (long long)p.m_tiles * p.n_tiles, chunk = kChunkBytes / ((long long)kTileN * 64 * p.groups) / 8 * 8;
     p.chunk = (int)(chunk < 8 ? 8 : chunk < p.n_tiles ? chunk : p.n_tiles);
     if (tiles > 0x7fffff) return hipErrorInvalidValue;      // a launch counts its threads in 32 bits
-    hipLaunchKernelGGL((mx_matmul_tile_kernel<FA, EXACT, WM, STAGES, PER_CU, TO>), dim3((unsigned int)tiles), dim3(kTileThreads), lds, stream, p);
+    hipLaunchKernelGGL((mx_matmul_tile_kernel<FA, WM, STAGES, PER_CU, TO>), dim3((unsigned int)tiles), dim3(kTileThreads), lds, stream, p);
     return hipGetLastError();
 }
 
@@ -657,16 +645,16 @@ template <int FA, bool EXACT, int WM, int STAGES, int PER_CU, typename TO> hipEr
 // fp32: n = 40000, 1.2 rounds, 30 / 32, 100003, 3.05 rounds, 65 / 70, 128000, 3.9 rounds, 90 / 83, 200000, 6.1 rounds, 131 / 120;
 // k = 2048, 100003 110 / 97; 2048 x 131072 x 4096 707 / 597).
 template <typename TO> hipError_t tiles_4bit(const TileArgs& p, hipStream_t stream) {
-    if (p.m <= 64) return launch_tiles<kMxFp4, false, 1, 3, 1, TO>(p, stream);
+    if (p.m <= 64) return launch_tiles<kMxFp4, 1, 3, 1, TO>(p, stream);
     const long long tall = (p.m + 255) / 256 * ((p.n + kTileN - 1) / kTileN);
     const bool few_last = tall < 4 * 256 && tall % 256 > 0 && tall % 256 <= 64;
-    if (p.m <= 128 || tall < 256 || (p.groups <= 8 && few_last)) return launch_tiles<kMxFp4, false, 2, 3, 2, TO>(p, stream);
-    return launch_tiles<kMxFp4, false, 4, 3, 1, TO>(p, stream);
+    if (p.m <= 128 || tall < 256 || (p.groups <= 8 && few_last)) return launch_tiles<kMxFp4, 2, 3, 2, TO>(p, stream);
+    return launch_tiles<kMxFp4, 4, 3, 1, TO>(p, stream);
 }
-template <bool EXACT, typename TO> hipError_t tiles_8bit(const TileArgs& p, hipStream_t stream) {
-    if (p.m <= 64) return launch_tiles<kMxFp8, EXACT, 1, 3, 1, TO>(p, stream);
-    if (p.m <= 128) return launch_tiles<kMxFp8, EXACT, 2, 3, 1, TO>(p, stream);
-    return launch_tiles<kMxFp8, EXACT, 4, 3, 1, TO>(p, stream);
+template <typename TO> hipError_t tiles_8bit(const TileArgs& p, hipStream_t stream) {
+    if (p.m <= 64) return launch_tiles<kMxFp8, 1, 3, 1, TO>(p, stream);
+    if (p.m <= 128) return launch_tiles<kMxFp8, 2, 3, 1, TO>(p, stream);
+    return launch_tiles<kMxFp8, 4, 3, 1, TO>(p, stream);
 }
 
 }  // namespace
@@ -696,7 +684,7 @@ hipError_t launch_mx_matmul(const void* a_values, const void* a_scales, int a_fo
         if (const hipError_t e = hipGetLastError(); e != hipSuccess) return e;
         const TileArgs p{a, b, as, bs, m, n, up(m, 256), up(n, 256), groups, 0, 0, 0, out, ld_out, whole, past};
         if (a_format == kMxFp4) return out_dtype == 0 ? tiles_4bit<float>(p, stream) : tiles_4bit<bf16_t>(p, stream);
-        return out_dtype == 0 ? tiles_8bit<true, float>(p, stream) : tiles_8bit<false, bf16_t>(p, stream);
+        return out_dtype == 0 ? tiles_8bit<float>(p, stream) : tiles_8bit<bf16_t>(p, stream);
     }
     const MatmulArgs p{a, static_cast<const unsigned char*>(a_scales), b, static_cast<const unsigned char*>(b_scales), m, n, groups, out, ld_out, whole};
     if (out_dtype == 0) return a_format == kMxFp4 ? rows_shaped<kMxFp4, float>(p, stream) : rows_shaped<kMxFp8, float>(p, stream);

@@ -225,12 +225,8 @@ def mx_matmul(a: MxRows, b: MxRows, dtype=None, out=None):
     32 bits; float32 unless `dtype` says bfloat16, or into `out`, a (m, n) GPU tensor
     with dense rows that do not overlap.  Rows of 1024 results and more start on 128
     bytes, as an index's rows do: where n is no multiple of that, the result is not
-    contiguous (its stride(0) is larger than n).
-
-    Sums of 4-bit rows are exact to 32 bits.  So are those of 8-bit rows in a float32
-    result; in a large bfloat16 one they come from the matrix instruction that
-    keeps about 16 bits of its largest product (2-norm error 1e-5 or less against
-    bfloat16's own 2e-3)."""
+    contiguous (its stride(0) is larger than n).  Sums are held in 32 bits whatever the
+    sizes and the result's type, and rounded once."""
     if b.format != "mxfp4":
         raise ValueError("mx_matmul wants its second operand in mxfp4")
     if a.d != b.d:

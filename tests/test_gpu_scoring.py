@@ -401,6 +401,58 @@ def test_matmul_far_scales(sc):
             assert torch.equal(sc.mx_matmul(a, b), (want * 2.0 ** 16).float())
 
 
+# few rows, and every tile shape
+UNEVEN = [(3, 300, 256), (290, 333, 1000), (64, 50001, 256), (128, 24001, 520), (300, 10111, 4096), (700, 24100, 300)]
+
+
+@pytest.mark.parametrize("out", ["float32", "bfloat16"])
+@pytest.mark.parametrize("fmt", ["mxfp8", "mxfp4"])
+def test_matmul_keeps_small_products_beside_large_ones_that_cancel(sc, fmt, out):
+    """Two pairs of large elements in each row of A whose products cancel exactly, the
+    smallest elements beside them.  All products are whole multiples of one unit whose sums in
+    any order stay below 2^24 of it: nothing may be rounded but the result."""
+    import torch
+    for i, (m, n, d) in enumerate(UNEVEN):
+        rng = np.random.default_rng(40 + i)
+        signed = lambda codes, f: codes + rng.integers(0, 2, size=codes.shape) * (8 if f == "mxfp4" else 128)  # noqa: E731
+        b = signed(rng.integers(1, 8, size=(n, orc.padded(d))), "mxfp4")
+        b_scales = np.full((n, orc.padded(d) // 32), 127, np.uint8)
+        a_scales = np.full((m, orc.padded(d) // 32), 127, np.uint8)
+        if fmt == "mxfp8":      # 1 .. 7 times 2^-9 beside 256 .. 448; the unit is 2^-10, 4 * 448 * 6 + 4096 * 7 * 2^-9 * 6 < 2^14
+            a = signed(rng.integers(1, 8, size=(m, orc.padded(d))), fmt)
+            a[:, [2, 40]] = signed(rng.integers(0x78, 0x7F, size=(m, 2)), fmt)
+        else:                   # 0.5 .. 6 beside 2^12 times that in two blocks; the unit is 1/4, 4 * 36 * 2^12 + 4096 * 36 < 2^20
+            a = signed(rng.integers(1, 8, size=(m, orc.padded(d))), fmt)
+            a[:, :128] = 0
+            a_scales[:, :4] = 127 + 12
+            a[:, [2, 40]] = signed(rng.integers(1, 8, size=(m, 2)), fmt)
+        a[:, [70, 101]] = a[:, [2, 40]]
+        b[:, [70, 101]] = b[:, [2, 40]] ^ 8
+        a[:, d:], b[:, d:] = 0, 0
+        a, b = a.astype(np.uint8), b.astype(np.uint8)
+        pa = sc.MxRows(torch.from_numpy(orc.pack(a, fmt)).cuda(), torch.from_numpy(a_scales).cuda(), d, fmt)
+        pb = sc.MxRows(torch.from_numpy(orc.pack(b, "mxfp4")).cuda(), torch.from_numpy(b_scales).cuda(), d, "mxfp4")
+        want = product(orc.mx_values(a, a_scales, fmt, d), orc.mx_values(b, b_scales, "mxfp4", d))
+        assert torch.equal(sc.mx_matmul(pa, pb, getattr(torch, out)), want.to(getattr(torch, out))), (m, n, d)
+
+
+@pytest.mark.parametrize("out", ["float32", "bfloat16"])
+@pytest.mark.parametrize("fmt", ["mxfp8", "mxfp4"])
+def test_matmul_of_columns_of_far_magnitudes(sc, fmt, out):
+    """As a model's hidden states are, a few columns far above the others.  An instruction
+    adds 32 products or 128 to the running sum; d / 32 + 128 additions in a row at most, each off
+    by one step of 32 bits (2 u) at most, and the result is rounded once."""
+    import torch
+    for i, (m, n, d) in enumerate(UNEVEN):
+        g = torch.Generator(device="cuda").manual_seed(i)
+        x = torch.randn(m, d, generator=g, device="cuda") * torch.exp(3 * torch.randn(1, d, generator=g, device="cuda"))
+        a, b = sc.mx_quantize(x, fmt), sc.mx_quantize(torch.randn(n, d, generator=g, device="cuda"))
+        va, vb = sc.mx_dequantize(a, torch.float32).double(), sc.mx_dequantize(b, torch.float32).double()
+        want, size = va @ vb.t(), va.abs() @ vb.abs().t()
+        got = sc.mx_matmul(a, b, getattr(torch, out)).double()
+        assert bool(((got - want).abs() <= 2 * (d / 32 + 128) * U * size + HALF_STEP[out] * want.abs() * (1 + 2.0 ** -7)).all()), (m, n, d)
+
+
 def test_matmul_result_rows_start_on_128_bytes(sc):
     import torch
     a, _ = stored(sc, 3, 64, "mxfp8", seed=1)
