@@ -228,6 +228,7 @@ template <int FA, int MT, int NT, int KS, typename TO> hipError_t launch_rows(co
 
 constexpr int kTileThreads = 512, kTileN = 256;
 constexpr int kTileMaxGroups = 16384;       // offsets within a tile fit 32 bits
+constexpr long long kMostWaveRows = 65535 * 64;     // of A, in the grid's y, where every wave is on its own
 // B's elements that all tiles of A are multiplied with before the next ones: they stay in the chip's 256 MB cache, and the
 // workgroups that run together write long pieces of few rows of out, which memory takes faster than short pieces of all rows
 // (measured, us, A's tiles running fastest / chunks of 24 MB / 40 MB / 96 MB / all of B at once: 511 x 100003 x 768 4 bits to
@@ -601,10 +602,22 @@ __global__ __launch_bounds__(kTileThreads, 2 * PER_CU) void mx_matmul_tile_kerne
 }
 
 
-// Tiles fill the chip from about 48 of them on; below, and for rows too long for their 32-bit offsets, every wave
-// on its own is faster (measured, k = 4096, 8 bits to fp32, microseconds, tiles / waves: 32 x 131072 100 / 110,
-// 16 x 131072 87 / 78, 256 x 16384 99 / 88, 512 x 16384 99 / 173, 512 x 4032 97 / 47, 1024 x 4032 98 / 88).
-bool takes_tiles(long long m, long long n, int groups) { return m * n > 3000000 && groups <= kTileMaxGroups; }
+// Tiles, or every wave on its own.  Up to 16 rows of A the waves are faster however many rows B has: they read it once, and
+// a tile has no use for most of its rows.  Above, a tile of 64, 128 or 256 rows of A takes its time however few of them there
+// are, and 8-bit rows are converted again by each of its waves, so that tiles pay from more results on the taller they are
+// (measured, us, tiles / waves, 8 bits to fp32 then 4 bits to fp32:
+//   1 x 4000000 x 768 537 / 314, 434 / 285; 16 x 4000000 x 768 537 / 426, 482 / 388; 16 x 131072 x 4096 88 / 79, 72 / 65
+//   32 x 50257 x 1024 16.5 / 15.7, 13.0 / 12.0; 64 x 16384 x 4096 37 / 29, 22 / 18; 32 x 50257 x 4096 46 / 54, 34 / 40;
+//   48 x 50257 x 1024 17 / 24, 13.5 / 15.6
+//   128 x 16384 x 4096 50 / 47, 24 / 31; 128 x 16384 x 1024 19 / 15, 13 / 10; 65 x 50257 x 1024 22 / 37, 15 / 21
+//   256 x 16384 x 4096 98 / 90, 26 / 57; 256 x 16384 x 1024 33 / 27, 14 / 17; 300 x 16384 x 4096 99 / 122, 27 / 79;
+//   512 x 4032 x 4096 96 / 47, 23 / 31; 512 x 4032 x 1024 32 / 15, 12 / 10; 1024 x 4032 x 4096 98 / 89, 25 / 57).
+// Rows too long for a tile's 32-bit offsets go to the waves, more row tiles than a launch counts to the tiles.
+bool takes_tiles(int format, long long m, long long n, int groups) {
+    if (m <= 16 || groups > kTileMaxGroups) return false;
+    if (m > kMostWaveRows) return true;
+    return m * n > (format == kMxFp4 ? 2000000 : m <= 64 ? 1500000 : m <= 128 ? 2250000 : 4500000);
+}
 
 template <int FA, int MT, typename TO> hipError_t rows_split(const MatmulArgs& p, hipStream_t stream) {
     // 16 rows of B a wave while that gives no CU a second workgroup, else 32; K split over four waves until there are
@@ -661,7 +674,8 @@ template <typename TO> hipError_t tiles_8bit(const TileArgs& p, hipStream_t stre
 
 long long mx_matmul_workspace(long long m, long long n, int d) {
     const int groups = mx_padded(d) / 128;
-    return takes_tiles(m, n, groups) ? (up(m, 256) + up(n, 256)) * groups * 4 : 0;
+    // of every format alike
+    return takes_tiles(kMxFp4, m, n, groups) || takes_tiles(kMxFp8, m, n, groups) ? (up(m, 256) + up(n, 256)) * groups * 4 : 0;
 }
 
 hipError_t launch_mx_matmul(const void* a_values, const void* a_scales, int a_format, long long m, const void* b_values,
@@ -672,7 +686,7 @@ hipError_t launch_mx_matmul(const void* a_values, const void* a_scales, int a_fo
     const int whole = ld_out % 4 == 0 && reinterpret_cast<uintptr_t>(out) % (4 * size) == 0;
     const auto* a = static_cast<const unsigned char*>(a_values);
     const auto* b = static_cast<const unsigned char*>(b_values);
-    if (takes_tiles(m, n, groups)) {
+    if (takes_tiles(a_format, m, n, groups)) {
         unsigned int* as = static_cast<unsigned int*>(workspace);
         unsigned int* bs = as + up(m, 256) * groups;
         // Results of 64 MB and more do not stay for their reader anyhow, and leave whole lines faster past the caches

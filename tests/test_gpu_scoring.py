@@ -453,6 +453,35 @@ def test_matmul_of_columns_of_far_magnitudes(sc, fmt, out):
         assert bool(((got - want).abs() <= 2 * (d / 32 + 128) * U * size + HALF_STEP[out] * want.abs() * (1 + 2.0 ** -7)).all()), (m, n, d)
 
 
+# around the sizes at which tiles take over from waves on their own, of 8- and of 4-bit rows: the last rows before
+# and the first ones behind, and few rows against very many
+CROSSINGS = [(1, 4_000_003, 100), (16, 400_001, 130), (17, 117_001, 130), (17, 118_001, 130), (64, 23_400, 200), (64, 23_500, 200),
+             (64, 31_300, 200), (65, 30_700, 130), (128, 17_500, 100), (128, 17_700, 300), (129, 34_800, 100), (129, 35_003, 200), (1100, 4100, 300),
+             (4_194_240, 1, 33), (4_194_241, 1, 33)]
+
+
+@pytest.mark.parametrize("fmt", ["mxfp8", "mxfp4"])
+def test_matmul_where_waves_and_tiles_meet(sc, fmt):
+    import torch
+    g = torch.Generator(device="cuda").manual_seed(2)
+
+    def whole(n, d, fmt):       # 0, 1, 2, 3, 4, 6 of both signs
+        few = torch.tensor([0, 2, 4, 5, 6, 7] if fmt == "mxfp4" else [0x00, 0x38, 0x40, 0x44, 0x48, 0x4C], dtype=torch.uint8, device="cuda")
+        codes = few[torch.randint(0, 6, (n, orc.padded(d)), device="cuda", generator=g)]
+        codes |= torch.randint(0, 2, codes.shape, device="cuda", generator=g, dtype=torch.uint8) << (3 if fmt == "mxfp4" else 7)
+        codes[:, d:] = 0
+        if fmt == "mxfp4":
+            codes = codes[:, ::2] | codes[:, 1::2] << 4
+        return sc.MxRows(codes.contiguous(), torch.full((n, orc.padded(d) // 32), 127, dtype=torch.uint8, device="cuda"), d, fmt)
+
+    for m, n, d in CROSSINGS:
+        a, b = whole(m, d, fmt), whole(n, d, "mxfp4")
+        want = sc.mx_dequantize(a, torch.float32).double() @ sc.mx_dequantize(b, torch.float32).double().t()
+        assert float(want.abs().max()) > 0
+        for dtype in (torch.float32, torch.bfloat16):
+            assert torch.equal(sc.mx_matmul(a, b, dtype), want.to(dtype)), (m, n, d)
+
+
 def test_matmul_result_rows_start_on_128_bytes(sc):
     import torch
     a, _ = stored(sc, 3, 64, "mxfp8", seed=1)

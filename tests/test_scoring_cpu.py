@@ -177,3 +177,14 @@ def test_constants_match_the_header():
         assert int(re.search(rf"#define {name} (\d+)", text).group(1)) == getattr(_native, name)
     for name in ("MTR_MX_FP4", "MTR_MX_FP8"):
         assert int(re.search(rf"{name} = (\d+)", text).group(1)) == getattr(_native, name)
+
+
+def test_products_of_few_rows_want_no_workspace():
+    """One to 16 rows take the kernel that reads B once, however many rows it has; a workspace for all
+    of B's scales would belong to the other one."""
+    from medical_rag_amd import _native
+    need = _native.lib().mtr_mx_matmul_workspace
+    for m, n, d in ((1, 4_000_000, 768), (1, 2 ** 29, 64), (12, 262144, 4096), (16, 262144, 2048), (16, 10_000_000, 1024)):
+        assert need(m, n, d) == 0, (m, n, d)
+    for m, n, d in ((17, 262144, 2048), (64, 131072, 4096), (2048, 131072, 4096), (2 ** 29, 1, 32), (5_000_000, 1, 32)):
+        assert need(m, n, d) > 0, (m, n, d)
