@@ -654,9 +654,11 @@ template <int FA, int WM, int STAGES, int PER_CU, typename TO> hipError_t launch
 
 // Tiles of 64, 128 or 256 rows of A.  4-bit rows have room for two workgroups of the 128-row tile a CU, whose starts and
 // ends overlap.  They take it where these weigh: with fewer tall tiles than CUs, or with short rows and a last round of tall
-// tiles (after few) that few CUs have one for (measured, us, two workgroups / tall: 1024 x 8192 x 4096 30 / 34; 511 rows, k = 768,
-// fp32: n = 40000, 1.2 rounds, 30 / 32, 100003, 3.05 rounds, 65 / 70, 128000, 3.9 rounds, 90 / 83, 200000, 6.1 rounds, 131 / 120;
-// k = 2048, 100003 110 / 97; 2048 x 131072 x 4096 707 / 597).
+// tiles (after few) that few CUs have one for.  Measured, time with two workgroups / with tall tiles, medians over m = 129 to
+// 2048 and k = 256 to 1024 to fp32 (bfloat16): 1 to 4 rounds, the last one at most a quarter full 0.92 (0.90), 88 (95) of 96
+// sizes below 1; the last one nearly full or full 1.02 (0.98); 4 to 7 rounds 1.03 (0.94); 8 and more 1.08 (1.02).  k = 1536 and
+// 2048: 1.02 (0.98) with such a last round, 1.13 (1.10) with a full one.  1024 x 8192 x 4096 in half a round 30 / 34 us,
+// 2048 x 131072 x 4096 707 / 597.
 template <typename TO> hipError_t tiles_4bit(const TileArgs& p, hipStream_t stream) {
     if (p.m <= 64) return launch_tiles<kMxFp4, 1, 3, 1, TO>(p, stream);
     const long long tall = (p.m + 255) / 256 * ((p.n + kTileN - 1) / kTileN);
