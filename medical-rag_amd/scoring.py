@@ -14,13 +14,15 @@ forward, as the encoder's does.
 
 Everything is enqueued on torch's current stream of the tensors' GPU without
 waiting, allocates through torch, and can be captured into a HIP graph.  The
-operators have no backward pass: they refuse inputs that record one.
+operators have no derivatives: they refuse inputs that record a backward pass or
+carry a forward-mode tangent.
 """
 from __future__ import annotations
 
 from collections import namedtuple
 
 import torch
+from torch.autograd import forward_ad
 
 from . import _native
 
@@ -47,12 +49,19 @@ def _code(dtype, what):
     return code
 
 
+def _no_derivative(t, what):
+    """Refuses a tensor whose derivatives would be lost without a word."""
+    if t.requires_grad and torch.is_grad_enabled():
+        raise ValueError(f"{what} has no backward pass: detach its inputs or call it under torch.no_grad()")
+    if forward_ad._current_level >= 0 and forward_ad.unpack_dual(t).tangent is not None:
+        raise ValueError(f"{what} has no forward derivative: pass the primal of its dual tensors")
+
+
 def _rows(x, what):
     """A (n, d) GPU tensor with dense rows (copied if its last dimension is strided)."""
     if not isinstance(x, torch.Tensor) or not x.is_cuda or x.dim() != 2:
         raise ValueError(f"{what} wants a 2-D GPU tensor")
-    if x.requires_grad and torch.is_grad_enabled():
-        raise ValueError(f"{what} has no backward pass: detach its inputs or call it under torch.no_grad()")
+    _no_derivative(x, what)
     return x if x.stride(1) == 1 or x.shape[1] < 2 else x.contiguous()
 
 
@@ -60,8 +69,7 @@ def _into(out, what):
     """Checks `out` of an operator without a backward pass, and tells autograd that it is overwritten."""
     if not isinstance(out, torch.Tensor) or not out.is_cuda:
         raise ValueError(f"{what}: out must be a GPU tensor")
-    if out.requires_grad and torch.is_grad_enabled():
-        raise ValueError(f"{what} has no backward pass: its out must not record one")
+    _no_derivative(out, what)
     if not out.is_inference():
         torch.autograd.graph.increment_version(out)
 
@@ -199,8 +207,7 @@ def rms_norm_mx(x, weight, eps: float = 1e-6, residual=None, format: str = "mxfp
     if (not isinstance(weight, torch.Tensor) or weight.shape != (d,) or weight.device != device
             or weight.dtype not in (dtype, torch.float32)):
         raise ValueError(f"rms_norm_mx wants a ({d},) weight of the rows' dtype or float32 on their GPU")
-    if weight.requires_grad and torch.is_grad_enabled():
-        raise ValueError("rms_norm_mx has no backward pass: detach its inputs or call it under torch.no_grad()")
+    _no_derivative(weight, "rms_norm_mx")
     if weight.stride(0) != 1:
         weight = weight.contiguous()
     h = None

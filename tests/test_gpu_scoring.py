@@ -770,3 +770,19 @@ def test_on_two_streams_at_once_and_twice_the_same(sc, n):
         for run in out:
             for a, b in zip(run, want):
                 assert torch.equal(a, b)
+
+
+def test_dual_tensors_are_refused(sc):
+    """The kernels would drop a forward-mode tangent without a word."""
+    import torch
+    from torch.autograd import forward_ad
+    x, w = rows(3, 64, "float32"), torch.ones(64, device="cuda")
+    packed = sc.mx_quantize(x)
+    with forward_ad.dual_level():
+        dual = forward_ad.make_dual(x, torch.ones_like(x))
+        for call in (lambda: sc.mx_quantize(dual), lambda: sc.rms_norm_mx(dual, w), lambda: sc.rms_norm_mx(x, w, 1e-6, dual),
+                     lambda: sc.rms_norm_mx(x, forward_ad.make_dual(w, torch.ones_like(w))), lambda: sc.token_logprobs(dual),
+                     lambda: sc.mx_dequantize(packed, out=dual), lambda: sc.mx_matmul(packed, packed, out=dual[:, :3])):
+            with pytest.raises(ValueError):
+                call()
+        check_quantized(sc.mx_quantize(forward_ad.unpack_dual(dual).primal), f64(x), "mxfp4")

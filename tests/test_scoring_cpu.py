@@ -188,3 +188,23 @@ def test_products_of_few_rows_want_no_workspace():
         assert need(m, n, d) == 0, (m, n, d)
     for m, n, d in ((17, 262144, 2048), (64, 131072, 4096), (2048, 131072, 4096), (2 ** 29, 1, 32), (5_000_000, 1, 32)):
         assert need(m, n, d) > 0, (m, n, d)
+
+
+def test_tensors_with_derivatives_are_refused():
+    from torch.autograd import forward_ad
+
+    from medical_rag_amd import scoring
+    x = torch.zeros(4, 64)
+    scoring._no_derivative(x, "it")
+    recorded = x.clone().requires_grad_()
+    with pytest.raises(ValueError, match="backward"):
+        scoring._no_derivative(recorded, "it")
+    with torch.no_grad():
+        scoring._no_derivative(recorded, "it")
+    with forward_ad.dual_level():
+        scoring._no_derivative(x, "it")
+        dual = forward_ad.make_dual(x, torch.ones_like(x))
+        for t in (dual, dual[1:], dual.t(), dual * 2):
+            with pytest.raises(ValueError, match="forward"):
+                scoring._no_derivative(t, "it")
+        scoring._no_derivative(forward_ad.unpack_dual(dual).primal, "it")
