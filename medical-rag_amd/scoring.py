@@ -66,10 +66,14 @@ def _rows(x, what):
 
 
 def _into(out, what):
-    """Checks `out` of an operator without a backward pass, and tells autograd that it is overwritten."""
+    """Checks `out` of an operator without derivatives."""
     if not isinstance(out, torch.Tensor) or not out.is_cuda:
         raise ValueError(f"{what}: out must be a GPU tensor")
     _no_derivative(out, what)
+
+
+def _written(out):
+    """Tells autograd that `out` has been overwritten: not before, as a refused call leaves it as it was."""
     if not out.is_inference():
         torch.autograd.graph.increment_version(out)
 
@@ -176,8 +180,8 @@ def mx_dequantize(rows: MxRows, dtype=None, out=None):
     """What microscaled rows stand for, as a (n, d) tensor of `dtype` (bfloat16, which
     holds every value exactly but the very smallest, unless given) or into `out`, a
     (n, d) GPU tensor with dense rows that do not overlap."""
-    n, d, device = rows._n, rows.d, rows.device
-    if out is None:
+    n, d, device, given = rows._n, rows.d, rows.device, out is not None
+    if not given:
         dtype = dtype or torch.bfloat16
         code = _code(dtype, "mx_dequantize")
         out = torch.empty_strided((n, d), (d, 1), dtype=dtype, device=device)
@@ -191,6 +195,8 @@ def mx_dequantize(rows: MxRows, dtype=None, out=None):
                                          _stream(device.index))
     if rc:
         _native.check(rc)
+    if given:
+        _written(out)
     return out
 
 
@@ -241,8 +247,8 @@ def mx_matmul(a: MxRows, b: MxRows, dtype=None, out=None):
     device = a.device
     if device != b.device:
         raise ValueError(f"operands are on {device} and {b.device}")
-    m, n = a._n, b._n
-    if out is None:
+    m, n, given = a._n, b._n, out is not None
+    if not given:
         dtype = dtype or torch.float32
         line = 32 if dtype == torch.float32 else 64
         out = torch.empty_strided((m, n), (n if n < 1024 else (n + line - 1) // line * line, 1), dtype=dtype, device=device)
@@ -259,6 +265,8 @@ def mx_matmul(a: MxRows, b: MxRows, dtype=None, out=None):
                            workspace.data_ptr() if need else None, need, device.index, _stream(device.index))
     if rc:
         _native.check(rc)
+    if given:
+        _written(out)
     return out
 
 

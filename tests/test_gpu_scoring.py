@@ -786,3 +786,26 @@ def test_dual_tensors_are_refused(sc):
             with pytest.raises(ValueError):
                 call()
         check_quantized(sc.mx_quantize(forward_ad.unpack_dual(dual).primal), f64(x), "mxfp4")
+
+
+def test_a_refused_out_counts_as_untouched(sc):
+    """A call refused for its out's shape, type or strides leaves a backward pass that saved it fine."""
+    import torch
+    packed = sc.mx_quantize(rows(3, 64, "float32"))
+    w = torch.ones(3, 65, device="cuda", requires_grad=True)
+    out = torch.ones(3, 65, device="cuda")
+    loss = (w * out).sum()
+    version = out._version
+    for call in (lambda: sc.mx_dequantize(packed, out=out), lambda: sc.mx_matmul(packed, packed, out=out), lambda: sc.mx_matmul(packed, packed, out=out[:, ::2]),
+                 lambda: sc.mx_dequantize(packed, torch.bfloat16, out=out[:, :64]), lambda: sc.mx_matmul(packed, packed, out=out[:1].expand(3, 65)[:, :3]),
+                 lambda: sc.mx_dequantize(packed, out=out[:1].expand(3, 65)[:, :64])):
+        with pytest.raises((ValueError, RuntimeError, TypeError)):
+            call()
+    half = torch.ones(3, 3, dtype=torch.float16, device="cuda")
+    with pytest.raises(TypeError):
+        sc.mx_matmul(packed, packed, out=half)
+    assert out._version == version and half._version == 0
+    loss.backward()
+    assert torch.equal(w.grad, out)
+    sc.mx_dequantize(packed, out=out[:, :64])
+    assert out._version > version
