@@ -58,10 +58,13 @@ def _no_derivative(t, what):
 
 
 def _rows(x, what):
-    """A (n, d) GPU tensor with dense rows (copied if its last dimension is strided)."""
+    """A (n, d) GPU tensor with dense rows (copied if its last dimension is strided, or if it stands for
+    the negative of what its memory holds, as the imaginary part of a conjugate does)."""
     if not isinstance(x, torch.Tensor) or not x.is_cuda or x.dim() != 2:
         raise ValueError(f"{what} wants a 2-D GPU tensor")
     _no_derivative(x, what)
+    if x.is_neg():
+        x = x.resolve_neg()
     return x if x.stride(1) == 1 or x.shape[1] < 2 else x.contiguous()
 
 
@@ -69,6 +72,8 @@ def _into(out, what):
     """Checks `out` of an operator without derivatives."""
     if not isinstance(out, torch.Tensor) or not out.is_cuda:
         raise ValueError(f"{what}: out must be a GPU tensor")
+    if out.is_neg():
+        raise ValueError(f"{what}: out stands for the negative of its memory")
     _no_derivative(out, what)
 
 
@@ -214,6 +219,8 @@ def rms_norm_mx(x, weight, eps: float = 1e-6, residual=None, format: str = "mxfp
             or weight.dtype not in (dtype, torch.float32)):
         raise ValueError(f"rms_norm_mx wants a ({d},) weight of the rows' dtype or float32 on their GPU")
     _no_derivative(weight, "rms_norm_mx")
+    if weight.is_neg():
+        weight = weight.resolve_neg()
     if weight.stride(0) != 1:
         weight = weight.contiguous()
     h = None

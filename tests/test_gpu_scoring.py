@@ -809,3 +809,22 @@ def test_a_refused_out_counts_as_untouched(sc):
     assert torch.equal(w.grad, out)
     sc.mx_dequantize(packed, out=out[:, :64])
     assert out._version > version
+
+
+def test_lazily_negated_tensors(sc):
+    """The imaginary part of a conjugate holds the other sign in memory; one column of it needs no copy for its strides."""
+    import torch
+    z = torch.complex(rows(5, 40, "float32", seed=1), rows(5, 40, "float32", seed=2)).conj()
+    for cols in (slice(0, 1), slice(0, 40)):
+        x = z[:, cols].imag
+        assert x.is_neg()
+        plain = x.resolve_neg().contiguous()
+        assert not plain.is_neg() and torch.equal(plain, x + 0)
+        check_quantized(sc.mx_quantize(x), f64(plain), "mxfp4")
+        for w, res in ((torch.ones(x.shape[1], device="cuda"), x), (z[0, cols].imag, plain)):
+            got, want = sc.rms_norm_mx(x, w, 1e-6, res), sc.rms_norm_mx(plain, w.resolve_neg().contiguous(), 1e-6, plain)
+            assert torch.equal(got[1], want[1]) and torch.equal(got[0].values, want[0].values) and torch.equal(got[0].scales, want[0].scales)
+        assert torch.equal(sc.token_logprobs(x, top_k=1).top_ids, sc.token_logprobs(plain, top_k=1).top_ids)
+        packed = sc.mx_quantize(plain)
+        with pytest.raises(ValueError):
+            sc.mx_dequantize(packed, out=z[:, cols].imag)
