@@ -293,7 +293,8 @@ int mtr_mx_dequantize(const void* dev_values, const void* dev_scales, int32_t fo
                       void* dev_out, int32_t dtype, int64_t ld, int32_t device_id, void* stream);
 /* h = x + residual, rounded to their type and written to dev_residual_out (dense
  * rows); then
- * h / sqrt(mean(h^2) + eps) * weight as microscaled rows.  dev_residual and
+ * h / sqrt(mean(h^2) + eps) * weight as microscaled rows (zeros of a zero row, also
+ * where eps is 0; a row whose squares overflow 32 bits gives zeros).  dev_residual and
  * dev_residual_out both NULL: h = x.  weight: d elements of the rows' type or
  * fp32.  d <= MTR_RMS_NORM_MAX_WIDTH. */
 #define MTR_RMS_NORM_MAX_WIDTH 65536

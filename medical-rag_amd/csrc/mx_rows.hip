@@ -137,7 +137,6 @@ __global__ __launch_bounds__(NT) void rms_norm_mx_kernel(const T* __restrict__ x
     const T* px = x + row * ld_x;
     const T* pr = RES ? residual + row * ld_res : nullptr;
     float h[NC][8];
-    float ss = 0.f;
 #pragma unroll
     for (int c = 0; c < NC; ++c) {
         const int col = (c * NT + tid) * 8;
@@ -157,20 +156,36 @@ __global__ __launch_bounds__(NT) void rms_norm_mx_kernel(const T* __restrict__ x
             else store_some<8>(residual_out + row * d + col, d - col, h[c]);
         }
     }
+    const auto sum_of_squares = [&] {
+        float ss = 0.f;
 #pragma unroll
-    for (int c = 0; c < NC; ++c)
+        for (int c = 0; c < NC; ++c)
 #pragma unroll
-        for (int i = 0; i < 8; ++i) ss = __builtin_fmaf(h[c][i], h[c][i], ss);
+            for (int i = 0; i < 8; ++i) ss = __builtin_fmaf(h[c][i], h[c][i], ss);
 #pragma unroll
-    for (int off = 32; off >= 1; off >>= 1) ss += __shfl_xor(ss, off, 64);
-    if constexpr (NT > 64) {
-        if ((tid & 63) == 0) red[tid >> 6] = ss;
-        __syncthreads();
-        ss = 0.f;
+        for (int off = 32; off >= 1; off >>= 1) ss += __shfl_xor(ss, off, 64);
+        if constexpr (NT > 64) {
+            if ((tid & 63) == 0) red[tid >> 6] = ss;
+            __syncthreads();
+            ss = 0.f;
 #pragma unroll
-        for (int w = 0; w < NT / 64; ++w) ss += red[w];
+            for (int w = 0; w < NT / 64; ++w) ss += red[w];
+        }
+        return ss;
+    };
+    float mean = sum_of_squares() / (float)d + eps;
+    // Squares that fall below what 32 bits hold, and no eps above them: once more with everything 2^100 times as large, where
+    // the largest sum, d 2^-100 of what it was, becomes 2^116 and the square of the smallest number 2^-98.  (The whole
+    // workgroup has the same mean.)
+    if (mean < 0x1p-100f) {
+        if constexpr (NT > 64) __syncthreads();     // everybody has read red
+#pragma unroll
+        for (int c = 0; c < NC; ++c)
+#pragma unroll
+            for (int i = 0; i < 8; ++i) h[c][i] *= 0x1p100f;
+        mean = sum_of_squares() / (float)d + eps * 0x1p100f * 0x1p100f;
     }
-    const float inv = 1.f / sqrtf(ss / (float)d + eps);
+    const float inv = mean == 0.f ? 0.f : 1.f / sqrtf(mean);    // a row of zeros stays one without an eps too
     const int padded = (d + kMxPad - 1) / kMxPad * kMxPad;
     const long long group0 = row * (padded / 128);
 #pragma unroll

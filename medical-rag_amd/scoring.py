@@ -210,7 +210,8 @@ def rms_norm_mx(x, weight, eps: float = 1e-6, residual=None, format: str = "mxfp
     h = x + residual in their dtype (None without a residual), the rows
     h / sqrt(mean(h^2) + eps) * weight.  x, residual: (n, d), one dtype; weight: (d,)
     of that dtype or float32.  Sums are in 32 bits: a row whose squares add up to more
-    than float32 holds comes back as zeros; d up to 65536."""
+    than float32 holds comes back as zeros (one whose squares are less than it holds does
+    not).  A zero row gives zeros, with eps 0 too.  d up to 65536."""
     x = _rows(x, "rms_norm_mx")
     n, d = x.shape
     dtype, device = x.dtype, x.device

@@ -828,3 +828,24 @@ def test_lazily_negated_tensors(sc):
         packed = sc.mx_quantize(plain)
         with pytest.raises(ValueError):
             sc.mx_dequantize(packed, out=z[:, cols].imag)
+
+
+@pytest.mark.parametrize("eps", [0.0, 1e-40, 1e-33, 1e-6])
+@pytest.mark.parametrize("dtype", ["float32", "bfloat16"])
+def test_rms_norm_of_rows_whose_squares_underflow(sc, dtype, eps):
+    """Squares below what 32 bits hold, down to the smallest numbers, with an eps above, among or below them; a zero
+    row gives zeros without an eps too.  Every width of a workgroup."""
+    import torch
+    for d in (1, 33, 512, 1000, 2049, 5000, 9000):
+        x = rows(8, d, "float32", seed=d, spread=0.0)
+        for i, scale in enumerate((1.0, 1e-14, 1e-16, 1e-19, 1e-22, 1e-30, 1e-38, 1e-42)):
+            x[i] *= scale
+        x = x.to(getattr(torch, dtype))
+        w = rows(1, d, "float32", seed=d + 1)[0]
+        x = x[(x != 0).any(dim=1)]      # one element may have rounded to zero
+        check_norm(sc, x, w, float(torch.tensor(eps)), None, "mxfp8")
+        check_norm(sc, x, w, float(torch.tensor(eps)), 0 * x, "mxfp4")
+        zero = torch.zeros(3, d, dtype=x.dtype, device="cuda")
+        zero[1] = x[0]
+        y = sc.mx_dequantize(sc.rms_norm_mx(zero, w, eps)[0], torch.float32)
+        assert (y[0] == 0).all() and (y[2] == 0).all() and torch.equal(y[1:2], sc.mx_dequantize(sc.rms_norm_mx(x[:1], w, eps)[0], torch.float32))
