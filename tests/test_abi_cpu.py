@@ -200,3 +200,17 @@ def test_rccl_stand_in_is_built_and_exports_what_the_library_resolves():
     lib = ctypes.CDLL(path)
     for name in ("ncclGetUniqueId", "ncclCommInitRank", "ncclCommDestroy", "ncclAllGather", "ncclGetErrorString"):
         assert hasattr(lib, name), name
+
+
+def test_every_object_is_compiled_without_packed_32_bit_float_instructions():
+    """Whatever flags a caller gives, and anew where the Makefile has changed since."""
+    import subprocess
+    csrc = os.path.join(ROOT, "medical-rag_amd", "csrc")
+    sources = [f for f in os.listdir(csrc) if f.endswith(".hip")]
+    for extra in ([], ["CXXFLAGS=-O1 -fPIC --offload-arch=gfx950"]):
+        plan = subprocess.run(["make", "-n", "-W", "Makefile", "-C", csrc, *extra, "all", "asan", "double"], check=True, capture_output=True, text=True).stdout
+        compiles = [line for line in plan.splitlines() if " -c " in line or "-x hip" in line]
+        for source in sources:
+            assert any(f" {source} " in line for line in compiles), f"{source} is not compiled anew"
+        for line in compiles:
+            assert "-target-feature -Xclang -packed-fp32-ops" in line, line
