@@ -214,3 +214,14 @@ def test_every_object_is_compiled_without_packed_32_bit_float_instructions():
             assert any(f" {source} " in line for line in compiles), f"{source} is not compiled anew"
         for line in compiles:
             assert "-target-feature -Xclang -packed-fp32-ops" in line, line
+
+
+def test_build_compiles_what_is_built_already(monkeypatch):
+    """A library that is there says nothing about the sources."""
+    import subprocess
+
+    import __graft_entry__ as entry
+    calls = []
+    monkeypatch.setattr(subprocess, "run", lambda command, **kw: calls.append(command))
+    entry.build()
+    assert len(calls) == 2 and all(c[0] == "make" and "-B" in c for c in calls)
