@@ -25,7 +25,7 @@ from . import scoring
 
 __all__ = ["ScoringHead", "page_scores", "rerank_pages", "rerank_hits"]
 
-MAX_LENGTH = 8192       # tokens of a page and a query together: what the index builder truncates pages to
+MAX_LENGTH = 8192       # tokens of a page and a query together, where the model takes as many: what the index builder truncates pages to
 SEPARATOR = "\n\n"      # between the page and the query
 
 
@@ -89,6 +89,13 @@ def _body(model):
     return body
 
 
+def _context(model) -> int | None:
+    """How many positions the model was made for; None where its configuration does not say."""
+    config = model.config.get_text_config() if hasattr(model.config, "get_text_config") else model.config
+    limit = getattr(config, "max_position_embeddings", None)
+    return limit if isinstance(limit, int) and limit > 0 else None
+
+
 def _sequences(page_ids: list, query_ids: list, separator_ids: list, start_ids: list, max_length: int):
     """Token lists [start, page, separator, query], the page cut so that the whole is at
     most max_length long, and where each one's query begins."""
@@ -103,7 +110,8 @@ _FORWARD = threading.Lock()
 
 
 def page_scores(query: str, texts: list, model, tokenizer, head: ScoringHead, batch_size: int = 8, max_length: int = MAX_LENGTH) -> list:
-    """Mean log probability of the query's tokens after each text, in nats."""
+    """Mean log probability of the query's tokens after each text, in nats.  Texts are
+    cut so that they and the query fit max_length tokens and the model's positions."""
     encode = lambda t: list(tokenizer(t, add_special_tokens=False)["input_ids"])  # noqa: E731
     query_ids = encode(query)
     if not query_ids or not texts:
@@ -113,7 +121,7 @@ def page_scores(query: str, texts: list, model, tokenizer, head: ScoringHead, ba
         start = tokenizer.eos_token_id
     # without any such token an empty page leaves nothing before the query's first one
     start_ids = [start] if start is not None else query_ids[:1]
-    rows, begins = _sequences([encode(t) for t in texts], query_ids, encode(SEPARATOR), start_ids, max_length)
+    rows, begins = _sequences([encode(t) for t in texts], query_ids, encode(SEPARATOR), start_ids, min(max_length, _context(model) or max_length))
     body, q = _body(model), len(query_ids)
     device = head.vocabulary.device
     captured, scores = [], []

@@ -1,5 +1,6 @@
 """Re-ranking: what needs no GPU (token arrangement, conventions, refusals)."""
 import logging
+from types import SimpleNamespace
 
 import numpy as np
 import pytest
@@ -58,3 +59,43 @@ def test_heads_that_compute_something_else_are_refused():
             ScoringHead.from_model(model)
     with pytest.raises(ValueError):     # a plain head, but not on a GPU
         ScoringHead.from_model(tiny_llama())
+
+
+class Characters:
+    """A tokenizer of one token a character."""
+    bos_token_id, cls_token_id, eos_token_id = 1, None, None
+
+    def __call__(self, text, add_special_tokens):
+        return {"input_ids": [2 + ord(c) % 60 for c in text]}
+
+
+class PlainHead:
+    """What ScoringHead does, in torch on any device."""
+
+    def __init__(self, model):
+        self.model = model
+        self.vocabulary = model.get_output_embeddings().weight
+
+    def token_logprobs(self, hidden, tokens):
+        from medical_rag_amd.scoring import TokenLogprobs
+        logits = self.model.get_output_embeddings()(self.model.model.norm(hidden))
+        return TokenLogprobs(torch.log_softmax(logits.double(), 1).gather(1, tokens[:, None]), None, None, None)
+
+
+def test_pages_are_cut_to_the_models_positions():
+    """The tiny model has 64: a longer page is scored as its beginning that fits, and no forward is longer."""
+    from medical_rag_amd import rerank
+    torch.manual_seed(0)
+    model = tiny_llama()
+    seen = []
+    model.model.register_forward_pre_hook(lambda module, args, kwargs: seen.append(kwargs["input_ids"].shape[1]), with_kwargs=True)
+    page, query = "".join(chr(97 + i * 7 % 26) for i in range(500)), "a query"
+    room = 64 - 1 - len(rerank.SEPARATOR) - len(query)
+    head = PlainHead(model)
+    long, cut, short = rerank.page_scores(query, [page, page[:room], page[:room - 20]], model, Characters(), head)
+    assert max(seen) == 64 and long == cut and cut != short
+    assert rerank.page_scores(query, [page], model, Characters(), head, max_length=40) == pytest.approx(
+        rerank.page_scores(query, [page[:room - 24]], model, Characters(), head))
+    bare = lambda **settings: SimpleNamespace(config=SimpleNamespace(**settings))  # noqa: E731
+    assert rerank._context(model) == 64 and rerank._context(bare(max_position_embeddings=9)) == 9
+    assert rerank._context(bare()) is None and rerank._context(bare(max_position_embeddings=None)) is None     # not every configuration says
