@@ -111,7 +111,8 @@ _FORWARD = threading.Lock()
 
 def page_scores(query: str, texts: list, model, tokenizer, head: ScoringHead, batch_size: int = 8, max_length: int = MAX_LENGTH) -> list:
     """Mean log probability of the query's tokens after each text, in nats.  Texts are
-    cut so that they and the query fit max_length tokens and the model's positions."""
+    cut so that they and the query fit max_length tokens and the model's positions; NaN
+    for all of them where the query alone does not."""
     encode = lambda t: list(tokenizer(t, add_special_tokens=False)["input_ids"])  # noqa: E731
     query_ids = encode(query)
     if not query_ids or not texts:
@@ -121,7 +122,11 @@ def page_scores(query: str, texts: list, model, tokenizer, head: ScoringHead, ba
         start = tokenizer.eos_token_id
     # without any such token an empty page leaves nothing before the query's first one
     start_ids = [start] if start is not None else query_ids[:1]
-    rows, begins = _sequences([encode(t) for t in texts], query_ids, encode(SEPARATOR), start_ids, min(max_length, _context(model) or max_length))
+    separator_ids, longest = encode(SEPARATOR), min(max_length, _context(model) or max_length)
+    if len(start_ids) + len(separator_ids) + len(query_ids) > longest:
+        logging.error(f"A query of {len(query_ids)} tokens does not fit the {longest} of the re-ranking model: its pages keep their order.")
+        return [float("nan")] * len(texts)
+    rows, begins = _sequences([encode(t) for t in texts], query_ids, separator_ids, start_ids, longest)
     body, q = _body(model), len(query_ids)
     device = head.vocabulary.device
     captured, scores = [], []
@@ -180,7 +185,8 @@ def rerank_pages(query: str, hits, pages, model_name: str, device: str = "cuda",
     """List positions `hits` of `pages` in the order of how likely the model finds the
     query after each page, and those scores (mean log probability a query token), both
     numpy arrays; equal scores keep their order, padding (position -1) is dropped.
-    When the model cannot be loaded the hits come back as they are, with NaN scores."""
+    When the model cannot be loaded, or the query has more tokens than it takes, the hits
+    come back as they are, with NaN scores."""
     hits = [int(h) for h in np.asarray(hits).reshape(-1) if 0 <= int(h) < len(pages)]
     if not hits:
         return np.empty(0, np.int64), np.empty(0, np.float32)

@@ -99,3 +99,24 @@ def test_pages_are_cut_to_the_models_positions():
     bare = lambda **settings: SimpleNamespace(config=SimpleNamespace(**settings))  # noqa: E731
     assert rerank._context(model) == 64 and rerank._context(bare(max_position_embeddings=9)) == 9
     assert rerank._context(bare()) is None and rerank._context(bare(max_position_embeddings=None)) is None     # not every configuration says
+
+
+def test_a_query_that_does_not_fit_keeps_its_own_order_and_the_others_theirs(monkeypatch):
+    from medical_rag_amd import rerank
+    torch.manual_seed(0)
+    model = tiny_llama()
+    monkeypatch.setattr(rerank, "_model_for", lambda name, device: (model, Characters(), PlainHead(model)))
+    pages = [{"index": i, "text": "page %d about it" % i} for i in range(5)]
+    long, fits = "x" * 64, "y" * (64 - 1 - len(rerank.SEPARATOR))
+    hits = {"first": ([0, 1, 2], None), long: ([4, -1, 2, 3], None), fits: ([1, 0], None), "last": ([3, 4], None)}
+    logging.disable(logging.CRITICAL)
+    try:
+        out = rerank.rerank_hits(hits, pages, "unused")
+    finally:
+        logging.disable(logging.NOTSET)
+    assert list(out) == list(hits)
+    assert out[long][0].tolist() == [4, 2, 3] and np.isnan(out[long][1]).all() and out[long][1].dtype == np.float32
+    for keyword in ("first", fits, "last"):
+        idx, scores = out[keyword]
+        want = dict(zip(hits[keyword][0], rerank.page_scores(keyword, [pages[i]["text"] for i in hits[keyword][0]], model, Characters(), PlainHead(model))))
+        assert [want[i] for i in idx.tolist()] == pytest.approx(scores.tolist()) and (np.diff(scores) <= 0).all()
