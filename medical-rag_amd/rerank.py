@@ -154,7 +154,7 @@ def page_scores(query: str, texts: list, model, tokenizer, head: ScoringHead, ba
     return torch.cat(scores).tolist()
 
 
-_MODEL = {"key": None, "model": None, "tokenizer": None, "head": None}
+_MODEL = {"key": None, "model": None, "tokenizer": None, "head": None, "refused": None}
 _LOADING = threading.Lock()
 
 
@@ -166,6 +166,8 @@ def _model_for(model_name: str, device: str):
 def _load(model_name: str, device: str):
     key = (model_name, device)
     if _MODEL["key"] == key:
+        if _MODEL["refused"]:
+            raise ValueError(_MODEL["refused"])
         return _MODEL["model"], _MODEL["tokenizer"], _MODEL["head"]
     from transformers import AutoModelForCausalLM, AutoTokenizer
     logging.info(f"Loading re-ranking model '{model_name}' onto device '{device}'.")
@@ -174,10 +176,14 @@ def _load(model_name: str, device: str):
         model = AutoModelForCausalLM.from_pretrained(model_name).to(device).eval()
     except Exception as exc:  # the encoder's soft failure (pipeline/utils/local_rag.py:34-37)
         logging.error(f"Failed to load re-ranking model '{model_name}': {exc}", exc_info=True)
-        _MODEL.update(key=None, model=None, tokenizer=None, head=None)
+        _MODEL.update(key=None, model=None, tokenizer=None, head=None, refused=None)
         return None, None, None
-    head = ScoringHead.from_model(model)
-    _MODEL.update(key=key, model=model, tokenizer=tokenizer, head=head)
+    try:
+        head = ScoringHead.from_model(model)
+    except ValueError as exc:       # remembered: loading the same model again would end here again
+        _MODEL.update(key=key, model=None, tokenizer=None, head=None, refused=str(exc))
+        raise
+    _MODEL.update(key=key, model=model, tokenizer=tokenizer, head=head, refused=None)
     return model, tokenizer, head
 
 

@@ -120,3 +120,25 @@ def test_a_query_that_does_not_fit_keeps_its_own_order_and_the_others_theirs(mon
         idx, scores = out[keyword]
         want = dict(zip(hits[keyword][0], rerank.page_scores(keyword, [pages[i]["text"] for i in hits[keyword][0]], model, Characters(), PlainHead(model))))
         assert [want[i] for i in idx.tolist()] == pytest.approx(scores.tolist()) and (np.diff(scores) <= 0).all()
+
+
+def test_a_refused_head_is_remembered(monkeypatch):
+    """The second call raises like the first and loads nothing; another model is loaded as ever."""
+    import transformers
+
+    from medical_rag_amd import rerank
+    loads = []
+
+    def load(name):
+        loads.append(name)
+        model = tiny_llama()
+        model.lm_head = torch.nn.Linear(32, 64, bias=True)
+        return model
+    monkeypatch.setattr(rerank, "_MODEL", dict.fromkeys(rerank._MODEL))
+    monkeypatch.setattr(transformers.AutoTokenizer, "from_pretrained", lambda name: Characters())
+    monkeypatch.setattr(transformers.AutoModelForCausalLM, "from_pretrained", load)
+    for name, so_far in (("one", 1), ("one", 1), ("two", 2), ("two", 2), ("one", 3)):
+        with pytest.raises(ValueError, match="bias"):
+            rerank._model_for(name, "cpu")
+        assert len(loads) == so_far
+    assert rerank._MODEL["model"] is None
