@@ -29,6 +29,9 @@ MAX_LENGTH = 8192       # tokens of a page and a query together, where the model
 SEPARATOR = "\n\n"      # between the page and the query
 
 
+_FORWARD = threading.Lock()     # one forward of a model at a time: the hook sees every one of them
+
+
 class ScoringHead:
     """The last steps of a causal language model on one GPU: root-mean-square norm with
     `norm_weight` and `eps`, then logits against `vocabulary` (MxRows in mxfp4, one row
@@ -62,6 +65,14 @@ class ScoringHead:
             want = x.double() / (x.double().square().mean() + eps).sqrt() * weight.double()
             if not torch.allclose(norm(x).double(), want, rtol=2e-2, atol=2e-2):
                 raise ValueError("the model's final norm is no plain root-mean-square norm")
+            # its logits of a few tokens against the same steps on the states in front of its norm: 2e-2 of the largest
+            # one is what roundings to 16 bits leave
+            ids = torch.arange(min(8, out.weight.shape[0]), device=weight.device)[None]
+            states, result = _states(model, model, ids)
+            logits = result.logits[0, -1].double()
+            want = torch.nn.functional.linear(norm(states[0, -1:]), out.weight)[0].double()
+            if logits.shape != want.shape or not bool(((logits - want).abs() <= 2e-2 * want.abs().max()).all()):
+                raise ValueError("the model's logits are not its final norm times its output embeddings")
             return cls(weight, eps, scoring.mx_quantize(out.weight.detach(), "mxfp4"))
 
     def logits(self, hidden, residual=None, dtype=torch.float32):
@@ -89,6 +100,19 @@ def _body(model):
     return body
 
 
+def _states(model, module, ids, **inputs):
+    """What goes into the norm that ends the decoder's body, (rows, tokens, width), and what `module` (the model
+    or its body) returns."""
+    captured = []
+    with _FORWARD, torch.no_grad():
+        hook = _body(model).norm.register_forward_pre_hook(lambda _, args: captured.append(args[0]))
+        try:
+            result = module(input_ids=ids, use_cache=False, **inputs)
+        finally:
+            hook.remove()
+    return captured[-1], result
+
+
 def _context(model) -> int | None:
     """How many positions the model was made for; None where its configuration does not say."""
     config = model.config.get_text_config() if hasattr(model.config, "get_text_config") else model.config
@@ -106,9 +130,6 @@ def _sequences(page_ids: list, query_ids: list, separator_ids: list, start_ids: 
     return rows, [len(r) - len(query_ids) for r in rows]
 
 
-_FORWARD = threading.Lock()
-
-
 def page_scores(query: str, texts: list, model, tokenizer, head: ScoringHead, batch_size: int = 8, max_length: int = MAX_LENGTH) -> list:
     """Mean log probability of the query's tokens after each text, in nats.  Texts are
     cut so that they and the query fit max_length tokens and the model's positions; NaN
@@ -122,35 +143,29 @@ def page_scores(query: str, texts: list, model, tokenizer, head: ScoringHead, ba
         start = tokenizer.eos_token_id
     # without any such token an empty page leaves nothing before the query's first one
     start_ids = [start] if start is not None else query_ids[:1]
-    separator_ids, longest = encode(SEPARATOR), min(max_length, _context(model) or max_length)
-    if len(start_ids) + len(separator_ids) + len(query_ids) > longest:
-        logging.error(f"A query of {len(query_ids)} tokens does not fit the {longest} of the re-ranking model: its pages keep their order.")
+    separator_ids, limit = encode(SEPARATOR), min(max_length, _context(model) or max_length)
+    if len(start_ids) + len(separator_ids) + len(query_ids) > limit:
+        logging.error(f"A query of {len(query_ids)} tokens does not fit the {limit} of the re-ranking model: its pages keep their order.")
         return [float("nan")] * len(texts)
-    rows, begins = _sequences([encode(t) for t in texts], query_ids, separator_ids, start_ids, longest)
+    rows, begins = _sequences([encode(t) for t in texts], query_ids, separator_ids, start_ids, limit)
     body, q = _body(model), len(query_ids)
     device = head.vocabulary.device
-    captured, scores = [], []
-    with _FORWARD, torch.no_grad():     # one thread at a time: the hook sees every forward of the model
-        hook = body.norm.register_forward_pre_hook(lambda module, args: captured.append(args[0]))
-        try:
-            tokens = torch.tensor(query_ids, device=device)
-            for lo in range(0, len(rows), batch_size):
-                part, at = rows[lo:lo + batch_size], begins[lo:lo + batch_size]
-                longest = max(map(len, part))
-                ids = torch.zeros((len(part), longest), dtype=torch.int64)
-                mask = torch.zeros((len(part), longest), dtype=torch.int64)
-                for i, r in enumerate(part):
-                    ids[i, :len(r)], mask[i, :len(r)] = torch.tensor(r), 1
-                captured.clear()
-                body(input_ids=ids.to(device), attention_mask=mask.to(device), use_cache=False)
-                hidden = captured[-1]
-                # the state at a position predicts the next token: from the one before the query to its last but one
-                where = (torch.tensor(at)[:, None] - 1 + torch.arange(q)[None]).to(device)
-                picked = hidden.gather(1, where[:, :, None].expand(-1, -1, hidden.shape[2])).reshape(-1, hidden.shape[2])
-                lp = head.token_logprobs(picked, tokens.repeat(len(part))).logprobs
-                scores.append(lp.reshape(len(part), q).mean(dim=1))
-        finally:
-            hook.remove()
+    scores = []
+    with torch.no_grad():
+        tokens = torch.tensor(query_ids, device=device)
+        for lo in range(0, len(rows), batch_size):
+            part, at = rows[lo:lo + batch_size], begins[lo:lo + batch_size]
+            longest = max(map(len, part))
+            ids = torch.zeros((len(part), longest), dtype=torch.int64)
+            mask = torch.zeros((len(part), longest), dtype=torch.int64)
+            for i, r in enumerate(part):
+                ids[i, :len(r)], mask[i, :len(r)] = torch.tensor(r), 1
+            hidden, _ = _states(model, body, ids.to(device), attention_mask=mask.to(device))
+            # the state at a position predicts the next token: from the one before the query to its last but one
+            where = (torch.tensor(at)[:, None] - 1 + torch.arange(q)[None]).to(device)
+            picked = hidden.gather(1, where[:, :, None].expand(-1, -1, hidden.shape[2])).reshape(-1, hidden.shape[2])
+            lp = head.token_logprobs(picked, tokens.repeat(len(part))).logprobs
+            scores.append(lp.reshape(len(part), q).mean(dim=1))
     return torch.cat(scores).tolist()
 
 

@@ -142,3 +142,28 @@ def test_a_refused_head_is_remembered(monkeypatch):
             rerank._model_for(name, "cpu")
         assert len(loads) == so_far
     assert rerank._MODEL["model"] is None
+
+
+def test_heads_are_compared_with_the_models_own_logits():
+    """Whatever a model does to its logits, named in its configuration or not."""
+    from transformers import LlamaForCausalLM
+
+    from medical_rag_amd.rerank import ScoringHead
+    torch.manual_seed(0)
+
+    def changed(change):
+        model = tiny_llama()
+        whole = LlamaForCausalLM.forward
+
+        def forward(*args, **kwargs):
+            result = whole(model, *args, **kwargs)
+            result.logits = change(result.logits)
+            return result
+        model.forward = forward
+        return model
+    for change in (lambda x: x / 2, lambda x: x * 1.1, lambda x: x[..., :40], lambda x: x + 0.1, lambda x: x * float("nan")):
+        with pytest.raises(ValueError, match="times its output embeddings"):
+            ScoringHead.from_model(changed(change))
+    for plain in (tiny_llama(), tiny_llama().to(torch.bfloat16), changed(lambda x: x.float())):     # then it is only not on a GPU
+        with pytest.raises(ValueError, match="GPU"):
+            ScoringHead.from_model(plain)
