@@ -7,10 +7,12 @@
     rocprofv3 --pmc SQ_BUSY_CU_CYCLES ... --kernel-trace --output-format csv -d DIR -- python3 profiles/scoring_head.py
     python3 profiles/scoring_head.py counters DIR/.../*_counter_collection.csv > profiles/scoring_head_pmc.json
 
+    python3 profiles/scoring_head.py rates > profiles/scoring_head_rates.json
+
 The first runs every case REPEATS times on inputs that lie in memory; the second
 writes, per case and kernel, the number of launches a call, the median time and what
 the case's bytes and operations make of it; the third the means of the counters that
-were collected, per kernel."""
+were collected, per kernel; the fourth what a large copy, fill and library product reach on the same card."""
 import csv
 import json
 import os
@@ -19,6 +21,13 @@ import sys
 
 sys.path.insert(0, os.path.dirname(os.path.dirname(os.path.abspath(__file__))))
 REPEATS, WARM = 12, 4
+
+
+def product(m, n, k, fmt, out):
+    size, width = {"float32": 4, "bfloat16": 2}[out], {"mxfp4": 17 / 32, "mxfp8": 33 / 32}[fmt]
+    return (f"product {m} x {n} x {k} {'8' if fmt == 'mxfp8' else '4'} x 4 bits to {'fp32' if size == 4 else 'bf16'}", "matmul", (m, n, k, fmt, out),
+            n * k * 17 / 32 + m * k * width + m * n * size, 2 * m * n * k)
+
 
 # name, operator, sizes, bytes a call has to move, operations of its products
 CASES = [
@@ -29,15 +38,17 @@ CASES = [
     ("read back 1M x 1000 8 bits to bf16", "dequantize", (1_000_000, 1000, "bfloat16", "mxfp8"), 1_000_000 * (2000 + 1024 + 32), 0),
     ("norm 1 x 4096 bf16 + residual to 8 bits", "norm", (1, 4096, "bfloat16"), 4096 * (6 + 2 + 1 + 1 / 32), 0),
     ("norm 8192 x 4096 bf16 + residual to 8 bits", "norm", (8192, 4096, "bfloat16"), 8192 * 4096 * (6 + 1 + 1 / 32), 0),
-    ("product 1 x 131072 x 4096 8 x 4 bits to fp32", "matmul", (1, 131072, 4096, "mxfp8", "float32"), 131072 * (4096 * 17 / 32 + 4), 2 * 131072 * 4096),
-    ("product 64 x 131072 x 4096 8 x 4 bits to fp32", "matmul", (64, 131072, 4096, "mxfp8", "float32"), 131072 * (4096 * 17 / 32 + 256), 2 * 64 * 131072 * 4096),
-    ("product 511 x 100003 x 768 4 x 4 bits to fp32", "matmul", (511, 100_003, 768, "mxfp4", "float32"), 100_003 * (768 * 17 / 32 + 511 * 4), 2 * 511 * 100_003 * 768),
-    ("product 2048 x 131072 x 4096 8 x 4 bits to fp32", "matmul", (2048, 131072, 4096, "mxfp8", "float32"), 131072 * (4096 * 17 / 32 + 8192), 2 * 2048 * 131072 * 4096),
-    ("product 2048 x 131072 x 4096 8 x 4 bits to bf16", "matmul", (2048, 131072, 4096, "mxfp8", "bfloat16"), 131072 * (4096 * 17 / 32 + 4096), 2 * 2048 * 131072 * 4096),
-    ("product 2048 x 131072 x 4096 4 x 4 bits to bf16", "matmul", (2048, 131072, 4096, "mxfp4", "bfloat16"), 131072 * (4096 * 17 / 32 + 4096), 2 * 2048 * 131072 * 4096),
+    *(product(*sizes) for sizes in (
+        (1, 131072, 4096, "mxfp8", "float32"), (1, 4_000_000, 768, "mxfp8", "float32"),
+        (32, 131072, 4096, "mxfp8", "float32"), (64, 131072, 4096, "mxfp8", "float32"), (250, 131072, 4096, "mxfp8", "float32"),     # a re-ranking batch
+        (300, 4032, 4096, "mxfp8", "float32"), (512, 4032, 4096, "mxfp8", "float32"), (1024, 4032, 4096, "mxfp8", "float32"),
+        (256, 16384, 4096, "mxfp8", "float32"), (512, 16384, 4096, "mxfp8", "float32"),
+        (64, 131072, 4096, "mxfp4", "float32"), (511, 100_003, 768, "mxfp4", "float32"), (1024, 4032, 4096, "mxfp4", "float32"),
+        (2048, 131072, 4096, "mxfp8", "float32"), (2048, 131072, 4096, "mxfp8", "bfloat16"), (2048, 131072, 4096, "mxfp4", "bfloat16"))),
     ("log probabilities 1 x 131072 fp32 top 20", "logprobs", (1, 131072, "float32", 20), 131072 * 4, 0),
     ("log probabilities 63 x 50257 fp16 top 5", "logprobs", (63, 50257, "float16", 5), 63 * 50257 * 2, 0),
     ("log probabilities 2048 x 131072 bf16 top 1", "logprobs", (2048, 131072, "bfloat16", 1), 2048 * 131072 * 2, 0),
+    ("log probabilities 250 x 131072 fp32", "logprobs", (250, 131072, "float32", 0), 250 * 131072 * 4, 0),
 ]
 
 
@@ -115,5 +126,26 @@ def counters(path):
     print(json.dumps({k: {c: round(sum(d.values()) / len(d)) for c, d in v.items()} for k, v in out.items()}, indent=1))
 
 
+def rates():
+    import torch
+
+    def median_us(f):
+        times = []
+        for i in range(WARM + REPEATS):
+            start, end = torch.cuda.Event(enable_timing=True), torch.cuda.Event(enable_timing=True)
+            start.record()
+            f()
+            end.record()
+            torch.cuda.synchronize()
+            times.append(start.elapsed_time(end) * 1e3)
+        return sorted(times[WARM:])[REPEATS // 2]
+    a, b = (torch.zeros(1 << 28, device="cuda") for _ in range(2))     # 1 GiB each
+    x, y = (torch.randn(8192, 8192, device="cuda", dtype=torch.bfloat16) for _ in range(2))
+    print(json.dumps({"copy 1 GiB, TB/s read and written": round(2 * 2 ** 30 / median_us(lambda: b.copy_(a)) / 1e6, 2),
+                      "fill 1 GiB, TB/s": round(2 ** 30 / median_us(lambda: b.fill_(1.0)) / 1e6, 2),
+                      "library product of two 8192 x 8192 bf16, PFLOP/s": round(2 * 8192 ** 3 / median_us(lambda: x @ y) / 1e9, 2)}, indent=1))
+
+
 if __name__ == "__main__":
-    {"summary": summary, "counters": counters}[sys.argv[1]](sys.argv[2]) if len(sys.argv) > 1 else run()
+    modes = {"summary": summary, "counters": counters, "rates": rates}
+    modes[sys.argv[1]](*sys.argv[2:]) if len(sys.argv) > 1 else run()
