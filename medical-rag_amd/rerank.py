@@ -69,7 +69,7 @@ class ScoringHead:
             # one is what roundings to 16 bits leave
             ids = torch.arange(min(8, out.weight.shape[0]), device=weight.device)[None]
             states, result = _states(model, model, ids)
-            logits = result.logits[0, -1].double()
+            logits = (result.logits if hasattr(result, "logits") else result[0])[0, -1].double()
             want = torch.nn.functional.linear(norm(states[0, -1:]), out.weight)[0].double()
             if logits.shape != want.shape or not bool(((logits - want).abs() <= 2e-2 * want.abs().max()).all()):
                 raise ValueError("the model's logits are not its final norm times its output embeddings")
@@ -110,6 +110,8 @@ def _states(model, module, ids, **inputs):
             result = module(input_ids=ids, use_cache=False, **inputs)
         finally:
             hook.remove()
+    if not captured:
+        raise ValueError(f"{type(model).__name__} does not go through its body's norm")
     return captured[-1], result
 
 

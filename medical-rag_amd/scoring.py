@@ -53,7 +53,7 @@ def _no_derivative(t, what):
     """Refuses a tensor whose derivatives would be lost without a word."""
     if t.requires_grad and torch.is_grad_enabled():
         raise ValueError(f"{what} has no backward pass: detach its inputs or call it under torch.no_grad()")
-    if forward_ad._current_level >= 0 and forward_ad.unpack_dual(t).tangent is not None:
+    if getattr(forward_ad, "_current_level", 0) >= 0 and forward_ad.unpack_dual(t).tangent is not None:
         raise ValueError(f"{what} has no forward derivative: pass the primal of its dual tensors")
 
 

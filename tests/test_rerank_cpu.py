@@ -167,3 +167,18 @@ def test_heads_are_compared_with_the_models_own_logits():
     for plain in (tiny_llama(), tiny_llama().to(torch.bfloat16), changed(lambda x: x.float())):     # then it is only not on a GPU
         with pytest.raises(ValueError, match="GPU"):
             ScoringHead.from_model(plain)
+
+
+def test_heads_of_models_that_return_tuples_or_pass_their_norm_by():
+    from types import MethodType
+
+    from medical_rag_amd.rerank import ScoringHead
+    whole = tiny_llama()
+    inner = whole.forward
+    whole.forward = lambda *args, **kwargs: (inner(*args, **kwargs).logits,)
+    with pytest.raises(ValueError, match="GPU"):        # a plain head, but not on a GPU
+        ScoringHead.from_model(whole)
+    around = tiny_llama()
+    around.forward = MethodType(lambda self, input_ids, use_cache: SimpleNamespace(logits=self.lm_head(self.model.embed_tokens(input_ids))), around)
+    with pytest.raises(ValueError, match="norm"):
+        ScoringHead.from_model(around)
